@@ -53,8 +53,8 @@ def _atomic_output(target: Path) -> Path:
 
 def build_hip(target: Path = HIP_LIBRARY) -> Path:
     tmp = _atomic_output(target)
-    _run([_hipcc(), *HIPCC_FLAGS, "-o", str(tmp), str(CSRC / "kernels.hip"), str(CSRC / "pool.cpp"),
-          str(CSRC / "hash.cpp")])
+    _run([_hipcc(), *HIPCC_FLAGS, "-o", str(tmp), str(CSRC / "kernels.hip"), str(CSRC / "append.hip"),
+          str(CSRC / "pool.cpp"), str(CSRC / "hash.cpp")])
     os.replace(tmp, target)
     return target
 

@@ -4,7 +4,7 @@
   the GPU (the reference's lookup contract, ``kvsnap/connector/dataplane.py:
   12-25``, with its ``KVSNAP_CUDA_LIBRARY`` override first).
 * ``kernel_library`` loads it once per path, types every kernel entry point
-  (``include/kvsnap_kernels.h``) and refuses another kernel ABI.
+  (``include/kvsnap_kernels.h``, ``include/kvsnap_attention.h``) and refuses another kernel ABI.
 * ``HostStaging`` holds the small pinned buffers that launch tables cross the
   host link in (see its docstring for why torch's pinned copies are not used).
 
@@ -72,6 +72,8 @@ KERNEL_SIGNATURES = {
     "kvsnap_stream_create": "int <- int size*",
     "kvsnap_stream_destroy": "int <- stream",
     "kvsnap_hold_stream": "int <- stream int",
+    "kvsnap_rotate": "int <- ptr i64 i64 ptr i64 i64 i64 int int int ptr stream",
+    "kvsnap_append": "int <- ptr ptr ptr ptr i64 i64 ptr i64 i64 ptr i64 i64 ptr i64 i64 i64 int int stream",
 }
 
 _loaded = {}

@@ -103,6 +103,28 @@ int kvsnap_append(const kvsnap_paged_layer* layer, const kvsnap_sequences* seque
                   int64_t query_head_stride, void* query_out, int64_t out_token_stride, int64_t out_head_stride,
                   int64_t tokens, int heads, int type, uintptr_t stream);
 
+/* Device bytes of scratch that kvsnap_attend needs for these sizes (0: none). */
+size_t kvsnap_attend_workspace_bytes(int64_t tokens, int n_seqs, int heads, int kv_heads, int width,
+                                     int64_t max_length, int64_t window);
+
+/* out[row, h] = the sum over the tokens t that a row sees of softmax(scale *
+ * query[row, h] . key[t]) value[t], for query and out of `tokens` rows of
+ * `heads` heads (a multiple of the layer's, consecutive ones sharing a key
+ * head) of type bf16 or fp16; a 16-bit cache is of the same type.  The row at
+ * position p of its sequence sees tokens 0..p, with window > 0 the last
+ * `window` of them; one that sees none has zeros (and a log sum of -inf).
+ * Softmax, sums and products' sums are fp32; weights are rounded to 16 bits
+ * before they meet the values (to two such terms for fp16 queries over an
+ * e4m3 cache), and an e4m3 cache's values are exact in bf16.  lse, or NULL:
+ * fp32 [tokens, heads], the natural logarithm of each row's sum of
+ * exponentials.  max_length, at least every sequence's length if it can be
+ * known, only shapes the launch.  workspace: 16-byte aligned scratch of
+ * kvsnap_attend_workspace_bytes bytes, used until the launch ends. */
+int kvsnap_attend(const kvsnap_paged_layer* layer, const kvsnap_sequences* sequences, const void* query,
+                  int64_t query_token_stride, int64_t query_head_stride, void* out, int64_t out_token_stride,
+                  int64_t out_head_stride, float* lse, int64_t tokens, int heads, int type, float scale,
+                  int64_t window, int64_t max_length, void* workspace, size_t workspace_bytes, uintptr_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -291,3 +291,63 @@ class PagedCache:
             self._layer_at, sequences, rotation, key.data_ptr(), key.stride(0), key.stride(1), value.data_ptr(),
             value.stride(0), value.stride(1), *rows, *out, tokens, heads, kind, stream)))
         return query_out
+
+    def attend(self, query, block_tables, lengths, *, query_starts=None, max_length=None, softmax_scale=None,
+               window=None, out=None, return_lse=False):
+        """Attention of a step's ``query`` rows ([rows, query heads, width], bfloat16 or float16) over their
+        sequences' tokens in the cache, the step's own included: ``[rows, query heads, width]`` of the query's type
+        (``out`` if given).
+
+        Query heads are a multiple of the cache's; consecutive ones share a key head.  A row at position p sees the
+        tokens 0 to p of its sequence, with ``window`` the last ``window`` of them, itself among them; a row that
+        sees none (a sequence of length 0) gets zeros.  Scores are ``softmax_scale`` (``width ** -0.5`` if None)
+        times the products; softmax and sums are fp32.  A 16-bit cache must have the query's type.
+
+        ``max_length``, the longest sequence's length if the caller knows it (the tables' width if None), only shapes
+        the launch.  With ``return_lse`` the result is ``(out, lse)``: fp32 ``[rows, query heads]`` natural
+        logarithms of the rows' sums of exponentials (-inf for a row that sees nothing), by which attention over
+        parts of the tokens can be joined.
+        """
+        import torch
+        _rows("query", query, None, None, self.width)
+        tokens, heads, _ = query.shape
+        dtype = query.dtype
+        kind = _TYPES.get(str(dtype))
+        if kind not in (0, 1) or (self._kind != 2 and kind != self._kind):
+            raise ValueError(f"queries must be bfloat16 or float16, a 16-bit cache's own type: {dtype} over "
+                             f"{self.cache.dtype}")
+        if heads % self.heads or not heads:
+            raise ValueError(f"{heads} query heads do not share the cache's {self.heads}")
+        if window is not None and window < 1:
+            raise ValueError("a window holds at least the row's own token")
+        scale = self.width ** -0.5 if softmax_scale is None else softmax_scale
+        if not 0 < scale < 1e30:
+            raise ValueError("softmax_scale must be positive and finite")
+        sequences, tensors = self._sequences(tokens, block_tables, lengths, query_starts)
+        named = block_tables.shape[1] * self.block_size
+        if max_length is None or max_length > named:
+            max_length = named
+        elif max_length < 0:
+            raise ValueError("max_length must not be negative")
+        if out is None:
+            out = torch.empty((tokens, heads, self.width), dtype=dtype, device=query.device)
+        else:
+            _rows("out", out, tokens, heads, self.width)
+            if out.dtype != dtype:
+                raise ValueError("out must have the query's type")
+        _on_gpu(self.device, query, out, *tensors)
+        lse = torch.empty((tokens, heads), dtype=torch.float32, device=self.device) if return_lse else None
+        lib = kernel_library()
+        window = window or 0
+        size = _workspace_bytes(lib, tokens, block_tables.shape[0], heads, self.heads, self.width, max_length, window)
+        scratch = torch.empty(size, dtype=torch.uint8, device=self.device) if size else None
+        _launch(self.device, lambda stream: _check(lib, lib.kvsnap_attend(
+            self._layer_at, sequences, query.data_ptr(), query.stride(0), query.stride(1), out.data_ptr(),
+            out.stride(0), out.stride(1), lse.data_ptr() if return_lse else None, tokens, heads, kind, scale, window,
+            max_length, scratch.data_ptr() if size else None, size, stream)))
+        return (out, lse) if return_lse else out
+
+
+@lru_cache(maxsize=256)
+def _workspace_bytes(lib, *sizes):
+    return lib.kvsnap_attend_workspace_bytes(*sizes)

@@ -53,8 +53,8 @@ def _atomic_output(target: Path) -> Path:
 
 def build_hip(target: Path = HIP_LIBRARY) -> Path:
     tmp = _atomic_output(target)
-    _run([_hipcc(), *HIPCC_FLAGS, "-o", str(tmp), str(CSRC / "kernels.hip"), str(CSRC / "append.hip"),
-          str(CSRC / "pool.cpp"), str(CSRC / "hash.cpp")])
+    sources = [str(CSRC / name) for name in ("kernels.hip", "append.hip", "attention.hip", "pool.cpp", "hash.cpp")]
+    _run([_hipcc(), *HIPCC_FLAGS, "-parallel-jobs=4", "-o", str(tmp), *sources])
     os.replace(tmp, target)
     return target
 

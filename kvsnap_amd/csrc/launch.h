@@ -55,7 +55,7 @@ inline void check_layer(const kvsnap_paged_layer& layer) {
 
 inline void check_sequences(const kvsnap_sequences& q, const kvsnap_paged_layer& layer) {
     require(q.n_seqs >= 0 && q.table_width >= 0 && q.table_stride >= 0, "negative table size");
-    require(int64_t(q.table_width) * layer.block_size < (int64_t(1) << 31), "the tables name 2^31 tokens or more");
+    require(int64_t(q.table_width) * layer.block_size < (int64_t(1) << 30), "the tables name 2^30 tokens or more");
     require(q.n_seqs == 0 || (q.lengths && (q.table_width == 0 || q.block_tables)), "the tables must be device pointers");
 }
 

@@ -43,9 +43,9 @@ struct Divider {
     }
 };
 
-// The values of an e8m0 byte: 2^(e - 127), 0 for e = 0 (2^-127 is below what fp32 holds normally), NaN for 255.
+// The value of an e8m0 byte: 2^(e - 127), NaN for 255.
 __device__ __forceinline__ float power_of(uint32_t e) {
-    return bits<float>(e == 255 ? 0x7fc00000u : e << 23);
+    return bits<float>(e == 255 ? 0x7fc00000u : e == 0 ? 0x00400000u : e << 23);
 }
 
 // Rows of sequence s, clamped to the `tokens` rows that there are: tables live in device memory, and a wrong one

@@ -35,7 +35,7 @@ POOL_ABI_VERSION = 2
 # ctypes types by the short names the signature table below uses.
 _TYPES = {
     "int": C.c_int, "ptr": C.c_void_p, "size": C.c_size_t, "u32": C.c_uint32, "u64": C.c_uint64,
-    "i64": C.c_int64, "str": C.c_char_p, "stream": C.c_size_t, "u64*": C.POINTER(C.c_uint64),
+    "i64": C.c_int64, "f32": C.c_float, "str": C.c_char_p, "stream": C.c_size_t, "u64*": C.POINTER(C.c_uint64),
     "ptr*": C.POINTER(C.c_void_p), "size*": C.POINTER(C.c_size_t), "void": None,
 }
 

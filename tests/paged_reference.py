@@ -83,7 +83,7 @@ def dequantised(cache, scales):
         side = side.float().double()
         if scales is not None:
             byte = scales[..., c].view(torch.uint8).double()
-            side = side * torch.where(byte == 0, 0.0, torch.where(byte == 255, math.nan, 2 ** (byte - 127)))[
+            side = side * torch.where(byte == 255, math.nan, 2 ** (byte - 127))[
                 :, None, :, None]
         out.append(side)
     return out

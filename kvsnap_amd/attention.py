@@ -338,8 +338,9 @@ class PagedCache:
         _on_gpu(self.device, query, out, *tensors)
         lse = torch.empty((tokens, heads), dtype=torch.float32, device=self.device) if return_lse else None
         lib = kernel_library()
-        window = window or 0
-        size = _workspace_bytes(lib, tokens, block_tables.shape[0], heads, self.heads, self.width, max_length, window)
+        window = min(window or 0, 1 << 30)
+        size = _workspace_bytes(lib, tokens, block_tables.shape[0], query_starts is not None, heads, self.heads,
+                                self.width, max_length, window)
         scratch = torch.empty(size, dtype=torch.uint8, device=self.device) if size else None
         _launch(self.device, lambda stream: _check(lib, lib.kvsnap_attend(
             self._layer_at, sequences, query.data_ptr(), query.stride(0), query.stride(1), out.data_ptr(),

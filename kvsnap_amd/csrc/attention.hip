@@ -30,12 +30,18 @@ struct Matrix<__bf16> {
     static __device__ __forceinline__ f32x4 mul16(Vec a, Vec b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
     }
+    static __device__ __forceinline__ f32x16 mul32(Vec a, Vec b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+    }
 };
 template <>
 struct Matrix<_Float16> {
     using Vec = half8_t;
     static __device__ __forceinline__ f32x4 mul16(Vec a, Vec b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ f32x16 mul32(Vec a, Vec b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
     }
 };
 
@@ -100,7 +106,24 @@ __device__ __forceinline__ float sum_across_groups(float x) {
     return bits<float>(quarters[0]) + bits<float>(quarters[1]);
 }
 
+__device__ __forceinline__ float max_across_halves(float x) {
+    auto halves = __builtin_amdgcn_permlane32_swap(bits<uint32_t>(x), bits<uint32_t>(x), false, false);
+    return __builtin_fmaxf(bits<float>(halves[0]), bits<float>(halves[1]));
+}
+__device__ __forceinline__ float sum_across_halves(float x) {
+    auto halves = __builtin_amdgcn_permlane32_swap(bits<uint32_t>(x), bits<uint32_t>(x), false, false);
+    return bits<float>(halves[0]) + bits<float>(halves[1]);
+}
+
+// One over a row's sum: 0 for a row that sees nothing, and NaN stays.
+__device__ __forceinline__ float over(float total) { return total > 0 ? 1.0f / total : total == 0 ? 0.0f : total; }
+
 // ----------------------------------------------------------------- a row alone
+
+// Tokens of a part, and parts that the longest row may have.
+struct Split {
+    int chunk, chunks;
+};
 
 struct Attend {
     kvsnap_paged_layer layer;
@@ -112,39 +135,42 @@ struct Attend {
     int tokens, heads, group;  // group: query heads that share a key head
     float scale;
     int window;                // 0: none
-    int chunk, chunks;         // tokens a workgroup takes, and parts a row may have
+    Split rows, tiles;         // of a row alone, and of a tile of rows
+    int parts;                 // the more of the two's: room in `part`
     int head_tiles;            // of 16 heads, of a key head's
-    Divider block_size;
-    float* part;               // [tokens, heads, chunks, width] sums, then [tokens, heads, chunks, 2] largest and sum
+    Divider block_size, group_size;
+    float* part;               // [tokens, heads, parts, width] sums, then [tokens, heads, parts, 2] largest and sum
 };
 
 constexpr int kTile = 32;         // tokens a wave takes at a time
 constexpr int kWaves = 4;         // of a workgroup, side by side along the tokens
 constexpr int kHeadTile = 16;     // query rows of a product
 
-// What a row sees: tokens [low, high) of its sequence.
+// What rows see, first to last: tokens [low, high) of their sequence, the first row at position `position`.
 struct Sight {
-    int sequence, low, high;
+    int low, high, position;
 };
 
-__device__ __forceinline__ Sight sight_of(const Attend& a, int row) {
-    Sight sight{row, 0, 0};
-    if (a.q.query_starts)
-        sight.sequence = find_sequence(a.q.n_seqs, row, [&](int s) { return int64_t(a.q.query_starts[s]); });
-    const Rows rows = rows_of(a.q, sight.sequence, a.tokens);
-    const int i = row - rows.first;
-    if (i < 0 || i >= rows.count) return Sight{-1, 0, 0};
-    const int length = length_of(a.q, sight.sequence), position = length - rows.count + i;
-    sight.low = a.window > 0 ? max(0, position + 1 - a.window) : 0;
-    sight.high = min(position + 1, named_of(a.q, length, a.layer.block_size));
-    return sight;
+__device__ __forceinline__ Sight sight_of(const Attend& a, int sequence, const Rows& rows, int first, int last) {
+    const int length = length_of(a.q, sequence), position = length - rows.count + first;
+    return Sight{a.window > 0 ? max(0, position + 1 - a.window) : 0,
+                 min(position + last - first + 1, named_of(a.q, length, a.layer.block_size)), position};
 }
 
-// Parts of a row's tokens, and the first token of part c: they start at the tile that holds the first seen token.
-// The last part that there is room for takes what is left.
-__device__ __forceinline__ int parts_of(const Attend& a, const Sight& sight) {
-    const int first = sight.low & ~(kTile - 1);
-    return sight.high <= sight.low ? 0 : min((sight.high - first + a.chunk - 1) / a.chunk, a.chunks);
+// Parts of what rows see: they start at the tile of tokens that holds the first seen token, and the last part that
+// there is room for takes what is left.
+template <int kTokens>
+__device__ __forceinline__ int parts_of(const Split& split, const Sight& sight) {
+    const int first = sight.low & ~(kTokens - 1);
+    return sight.high <= sight.low ? 0 : min((sight.high - first + split.chunk - 1) / split.chunk, split.chunks);
+}
+
+// Where a part's sums of a row's head are, and its largest score and total.
+__device__ __forceinline__ float* part_sums(const Attend& a, int64_t row_head, int part) {
+    return a.part + (row_head * a.parts + part) * a.layer.width;
+}
+__device__ __forceinline__ float* part_totals(const Attend& a, int64_t row_head, int part) {
+    return a.part + int64_t(a.tokens) * a.heads * a.parts * a.layer.width + (row_head * a.parts + part) * 2;
 }
 
 // One wave's loads of a tile: K's rows for the first product and V's for the second.
@@ -177,12 +203,12 @@ __global__ __launch_bounds__(kWaves * 64) void attend_row_kernel(Attend a) {
     job /= kv_heads;
     const int head_tile = job % a.head_tiles;
     job /= a.head_tiles;
-    const int part = job % a.chunks;
-    const int row = job / a.chunks;
-
-    const Sight sight = sight_of(a, row);
-    if (sight.sequence < 0) return;                         // padding
-    const int parts = parts_of(a, sight);
+    const int part = job % a.rows.chunks, sequence = job / a.rows.chunks;
+    const Rows rows = rows_of(a.q, sequence, a.tokens);
+    if (rows.count != 1) return;                            // tiles take sequences of more rows
+    const int row = rows.first;
+    const Sight sight = sight_of(a, sequence, rows, 0, 0);
+    const int parts = parts_of<kTile>(a.rows, sight);
     if (part >= max(parts, 1)) return;                      // the first part of a row that sees nothing writes zeros
 
     const int width = a.layer.width, size = a.layer.block_size;
@@ -216,9 +242,9 @@ __global__ __launch_bounds__(kWaves * 64) void attend_row_kernel(Attend a) {
     float top = -__builtin_inff(), total = 0;
     const float factor = a.scale * kLog2e;
 
-    const int base = (sight.low & ~(kTile - 1)) + part * a.chunk;
-    const int stop = part == a.chunks - 1 ? sight.high : min(sight.high, base + a.chunk);
-    const int32_t* const table = a.q.block_tables + sight.sequence * a.q.table_stride;
+    const int base = (sight.low & ~(kTile - 1)) + part * a.rows.chunk;
+    const int stop = part == a.rows.chunks - 1 ? sight.high : min(sight.high, base + a.rows.chunk);
+    const int32_t* const table = a.q.block_tables + sequence * a.q.table_stride;
     const char* const keys = static_cast<const char*>(a.layer.key) + kv_head * a.layer.head_stride * kBytes;
     const char* const values = static_cast<const char*>(a.layer.value) + kv_head * a.layer.head_stride * kBytes;
     const uint8_t* const scales = kEight ? a.layer.scales + kv_head * a.layer.scale_head_stride : nullptr;
@@ -440,74 +466,474 @@ __global__ __launch_bounds__(kWaves * 64) void attend_row_kernel(Attend a) {
         }
         const int64_t index = int64_t(row) * a.heads + first_head + head;
         if (parts > 1) {
-            float* const to = a.part + (index * a.chunks + part) * width + d;
+            float* const to = part_sums(a, index, part) + d;
             to[0] = x;
             to[1] = y;
             if (d == 0) {
-                float* const about = a.part + int64_t(a.tokens) * a.heads * a.chunks * width +
-                                     (index * a.chunks + part) * 2;
+                float* const about = part_totals(a, index, part);
                 about[0] = most;
                 about[1] = all;
             }
         } else {
-            const float over = all > 0 ? 1.0f / all : all == 0 ? 0.0f : all;    // NaN stays
+            const float share = over(all);
             Q* const to = static_cast<Q*>(a.out) + row * a.out_token_stride +
                           (first_head + head) * a.out_head_stride + d;
-            to[0] = static_cast<Q>(x * over);
-            to[1] = static_cast<Q>(y * over);
+            to[0] = static_cast<Q>(x * share);
+            to[1] = static_cast<Q>(y * share);
             if (a.lse && d == 0) a.lse[index] = most * a.scale + __builtin_logf(all);
         }
     }
 }
 
-// The parts of a row's head, joined: a workgroup's threads take values along the row and parts in turn.
+// ----------------------------------------------------------------- rows in tiles
+
+constexpr int kTileRows = 128;    // rows of a workgroup: (token, head) pairs that share a key head, heads fastest
+constexpr int kTileWaves = 4;     // 32 rows each, the columns of a product
+constexpr int kTileTokens = 64;   // tokens staged at a time
+
+// The tile of a sequence's rows that starts at pair `first`: the tokens of its first and last pair.
+__device__ __forceinline__ Sight tile_sight(const Attend& a, int sequence, const Rows& rows, int first) {
+    const int last = min(first + kTileRows, rows.count * a.group) - 1;
+    return sight_of(a, sequence, rows, a.group_size.divide(first), a.group_size.divide(last));
+}
+
+// Whether a pair of 16-bit values holds one that is not finite (`ones`: the type's exponent bits, twice).
+template <typename T>
+__device__ __forceinline__ uint32_t not_finite(uint32_t word) {
+    constexpr uint32_t ones = sizeof(T) == 2 && __is_same(T, _Float16) ? 0x7c00u : 0x7f80u;
+    return ((word & ones) == ones ? 0xffffu : 0u) | ((word >> 16 & ones) == ones ? 0xffff0000u : 0u);
+}
+
+// A prompt's rows: 128 of them by 64 tokens at a time, K and V staged in LDS in the products' type, two buffers deep:
+// the next tokens' loads are under way while the present ones' products run, and one barrier parts the two.
+//
+// K's rows are 16 bytes longer than the values (an odd number of 16-byte pieces: 16-byte reads down a column of rows
+// meet every bank), V's 32 (four rows' 32-byte pieces side by side, what one transposing read takes).
+template <typename Q, bool kEight, int kD>
+__global__ __launch_bounds__(kTileWaves * 64, kD <= 128 ? 2 : 1) void attend_tile_kernel(Attend a) {
+    using T = typename Shape<Q, kEight>::T;
+    using Vec = typename Matrix<T>::Vec;
+    constexpr int kTerms = Shape<Q, kEight>::kTerms;
+    constexpr int kBytes = kEight ? 1 : 2;
+    constexpr int kSteps = kD / 16, kBlocks = kD / 32;
+    constexpr int kPieces = kD / 8;                         // of eight values, of a row
+    constexpr int kLoads = kTileTokens * kPieces / (kTileWaves * 64);
+    constexpr int kKeyRow = kD * 2 + 16, kValueRow = kD * 2 + 32;
+    constexpr int kStage = kTileTokens * (kKeyRow + kValueRow);
+    constexpr uint32_t kNowhere = ~0u;
+    __shared__ __attribute__((aligned(16))) char stage[2 * kStage];
+    __shared__ uint32_t odd[3][2];                          // tokens with a value that is not finite, by turns
+
+    const int kv_heads = a.layer.kv_heads;
+    uint32_t job = blockIdx.x;
+    const int kv_head = job % kv_heads;
+    job /= kv_heads;
+    const int part = job % a.tiles.chunks;
+    // Later tiles see more tokens: they go first.
+    const int64_t slot_of_all = gridDim.x / kv_heads / a.tiles.chunks - 1 - job / a.tiles.chunks;
+    // Sequence s has slots from query_starts[s] * group / 128 + s on: n rows have at most n * group / 128 + 1 tiles.
+    const auto slots = [&](int s) {
+        return int64_t(min(max(a.q.query_starts[s], 0), a.tokens)) * a.group / kTileRows + s;
+    };
+    const int sequence = find_sequence(a.q.n_seqs, slot_of_all, slots);
+    const Rows rows = rows_of(a.q, sequence, a.tokens);
+    if (rows.count < 2) return;                             // none, or a row alone
+    const int64_t first_pair = (slot_of_all - slots(sequence)) * kTileRows;
+    const int pairs = rows.count * a.group;
+    if (first_pair < 0 || first_pair >= pairs) return;
+    const int pair0 = static_cast<int>(first_pair);
+    const Sight sight = tile_sight(a, sequence, rows, pair0);
+    const int parts = parts_of<kTileTokens>(a.tiles, sight);
+    if (part >= max(parts, 1)) return;
+
+    const int width = a.layer.width;
+    const int thread = threadIdx.x, lane = thread & 63, wave = __builtin_amdgcn_readfirstlane(thread >> 6);
+    const int column = lane & 31, half = lane >> 5;
+
+    // This lane's row, and the positions of the wave's first and last.
+    const int pair = pair0 + wave * 32 + column;
+    const bool real = pair < pairs;
+    const int token_of = a.group_size.divide(min(pair, pairs - 1)), head_of = min(pair, pairs - 1) - token_of * a.group;
+    const int place0 = length_of(a.q, sequence) - rows.count;
+    const int position = place0 + token_of;
+    const int wave_first = pair0 + wave * 32;
+    const bool idle = wave_first >= pairs;
+    const int low_position = place0 + static_cast<int>(a.group_size.divide(min(wave_first, pairs - 1)));
+    const int high_position = place0 + static_cast<int>(a.group_size.divide(min(wave_first + 31, pairs - 1)));
+    const int after = a.window > 0 ? position - a.window : -1;      // the row sees tokens behind this one, up to its own
+    const int64_t row = rows.first + token_of;
+    const int head = kv_head * a.group + head_of;
+
+    Vec q[kSteps][kTerms];
+    {
+        const Q* const from = static_cast<const Q*>(a.query) + row * a.query_token_stride + head * a.query_head_stride;
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            const int at = s * 16 + half * 8;
+            typename Matrix<Q>::Vec x{};
+            if (real && at < width) x = *reinterpret_cast<const typename Matrix<Q>::Vec*>(from + at);
+            if constexpr (kTerms == 1) {
+                q[s][0] = x;
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) two_terms(static_cast<float>(x[i]), q[s][0], q[s][1], i);
+            }
+        }
+    }
+
+    const int base = (sight.low & ~(kTileTokens - 1)) + part * a.tiles.chunk;
+    const int stop = part == a.tiles.chunks - 1 ? sight.high : min(sight.high, base + a.tiles.chunk);
+    const int32_t* const table = a.q.block_tables + sequence * a.q.table_stride;
+    const char* const keys = static_cast<const char*>(a.layer.key) + kv_head * a.layer.head_stride * kBytes;
+    const char* const values = static_cast<const char*>(a.layer.value) + kv_head * a.layer.head_stride * kBytes;
+    const uint8_t* const scales = kEight ? a.layer.scales + kv_head * a.layer.scale_head_stride : nullptr;
+
+    // Lane i's token of the 64 at `token`: where its rows are, in 16 bytes, and its block's scales.
+    struct Place {
+        uint32_t at;
+        float k_scale, v_scale;
+    };
+    const auto place_of = [&](int token) {
+        const int mine = token + lane;
+        Place place{kNowhere, 0, 0};
+        const uint32_t page = a.block_size.divide(mine);
+        if (mine < sight.low || mine >= stop || page >= static_cast<uint32_t>(a.q.table_width)) return place;
+        const int block = table[page];
+        if (static_cast<uint32_t>(block) >= static_cast<uint64_t>(a.layer.blocks)) return place;
+        const int slot = mine - page * a.block_size.d;
+        place.at = static_cast<uint32_t>((block * a.layer.block_stride + slot * a.layer.token_stride) * kBytes >> 4);
+        if constexpr (kEight) {
+            const uint8_t* const scale = scales + block * a.layer.scale_block_stride;
+            place.k_scale = power_of(scale[0]);
+            place.v_scale = power_of(scale[a.layer.scale_side_stride]);
+        }
+        return place;
+    };
+    // A thread's pieces of a stage: piece thread + 256 i, in the order of rows.
+    uint32_t k_words[kLoads][kEight ? 2 : 4], v_words[kLoads][kEight ? 2 : 4];
+    const auto load = [&](const Place& place) {
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const int index = thread + i * kTileWaves * 64;
+            const int token = index / kPieces, piece = index - token * kPieces;
+            const uint32_t at = __shfl(place.at, token);
+#pragma unroll
+            for (int w = 0; w < (kEight ? 2 : 4); ++w) k_words[i][w] = v_words[i][w] = 0;
+            if (at != kNowhere && piece * 8 < width) {
+                const int64_t offset = (int64_t(at) << 4) + piece * 8 * kBytes;
+                load_words<kEight ? 2 : 4>(keys + offset, k_words[i]);
+                load_words<kEight ? 2 : 4>(values + offset, v_words[i]);
+            }
+        }
+    };
+    const auto store = [&](const Place& place, char* to, bool ragged, uint32_t* odd_tokens) {
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const int index = thread + i * kTileWaves * 64;
+            const int token = index / kPieces, piece = index - token * kPieces;
+            u32x4 k, v;
+            if constexpr (kEight) {
+                const float k_scale = __shfl(place.k_scale, token), v_scale = __shfl(place.v_scale, token);
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    k[w] = two_bf16(k_words[i][w >> 1], k_scale, w & 1);
+                    v[w] = two_bf16(v_words[i][w >> 1], v_scale, w & 1);
+                }
+            } else {
+#pragma unroll
+                for (int w = 0; w < 4; ++w) k[w] = k_words[i][w], v[w] = v_words[i][w];
+            }
+            if (ragged) {
+                // Some rows do not see some of these tokens, and a weight of 0 does not hide NaN: such values stay
+                // out of the product and are added apart, for the rows that see them.
+                uint32_t any = 0;
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    const uint32_t bad = not_finite<T>(v[w]);
+                    any |= bad;
+                    v[w] &= ~bad;
+                }
+                if (any) atomicOr(&odd_tokens[token >> 5], 1u << (token & 31));
+            }
+            *reinterpret_cast<u32x4*>(to + token * kKeyRow + piece * 16) = k;
+            *reinterpret_cast<u32x4*>(to + kTileTokens * kKeyRow + token * kValueRow + piece * 16) = v;
+        }
+    };
+    // Whether some of the workgroup's rows see some of the 64 tokens and not others.
+    const int last_position = place0 + static_cast<int>(a.group_size.divide(min(pair0 + kTileRows, pairs) - 1));
+    const auto is_ragged = [&](int token) {
+        return token + kTileTokens - 1 > sight.position || (a.window > 0 && token <= last_position - a.window);
+    };
+
+    f32x16 sum[kBlocks];
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sum[b][i] = 0;
+    float top = -__builtin_inff(), total = 0;
+    const float factor = a.scale * kLog2e;
+
+    if (thread < 6) odd[thread >> 1][thread & 1] = 0;
+    Place place = place_of(base);
+    load(place);
+    Place next = place_of(base + kTileTokens);
+    __syncthreads();
+    store(place, stage, is_ragged(base), odd[0]);
+    uint64_t valid = __ballot(place.at != kNowhere);
+    __syncthreads();
+
+    int turn = 0;                                           // of three: whose odd tokens
+    int now = 0;                                            // the buffer of these tokens
+    for (int token = base; token < stop; token += kTileTokens) {
+        const bool more = token + kTileTokens < stop;
+        const int turn_next = turn == 2 ? 0 : turn + 1, turn_after = turn_next == 2 ? 0 : turn_next + 1;
+        if (thread < 2) odd[turn_after][thread] = 0;
+        Place after_next{kNowhere, 0, 0};
+        if (more) {
+            load(next);
+            after_next = place_of(token + 2 * kTileTokens);
+        }
+
+        const bool apart = idle || token > high_position || (a.window > 0 && token + kTileTokens <= low_position - a.window + 1);
+        if (!apart) {
+            const bool whole = valid == ~uint64_t(0) && token + kTileTokens - 1 <= low_position &&
+                               (a.window <= 0 || token > high_position - a.window);
+            f32x16 score[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) score[h][i] = 0;
+                const char* const from = stage + now + (32 * h + column) * kKeyRow + half * 16;
+#pragma unroll
+                for (int s = 0; s < kSteps; ++s) {
+                    const Vec k = *reinterpret_cast<const Vec*>(from + s * 32);
+#pragma unroll
+                    for (int t = 0; t < kTerms; ++t) score[h] = Matrix<T>::mul32(k, q[s][t], score[h]);
+                }
+            }
+            if (!whole) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const int at = 32 * h + 8 * (i >> 2) + 4 * half + (i & 3);
+                        const bool sees = token + at <= position && token + at > after && (valid >> at & 1);
+                        score[h][i] = sees ? score[h][i] : -__builtin_inff();
+                    }
+            }
+            float most = -__builtin_inff();
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) most = __builtin_fmaxf(most, score[h][i]);
+            most = max_across_halves(most);
+            if (__ballot(most > top)) {
+                const float grown = __builtin_fmaxf(top, most);
+                const float shrink = top == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((top - grown) * factor);
+                total *= shrink;
+#pragma unroll
+                for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) sum[b][i] *= shrink;
+                top = grown;
+            }
+            const float against = top == -__builtin_inff() ? 0.0f : top * factor;
+            Vec p[4][kTerms];
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    score[h][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(score[h][i], factor, -against));
+                    total += score[h][i];
+                    const int t = 2 * h + (i >> 3);
+                    if constexpr (kTerms == 2) two_terms(score[h][i], p[t][0], p[t][1], i & 7);
+                    else p[t][0][i & 7] = static_cast<T>(score[h][i]);
+                }
+            // V^T's operand: the four tokens that S^T left side by side, for 16 values by 16 lanes, in one
+            // transposing read.
+            const char* const from = stage + now + kTileTokens * kKeyRow + (4 * half + ((lane & 15) >> 2)) * kValueRow +
+                                     ((lane >> 4 & 1) * 16 + (lane & 3) * 4) * 2;
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int b = 0; b < kBlocks; ++b) {
+                    u32x4 words;
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const auto four = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                            (__attribute__((address_space(3))) short4_t*)(from + (16 * t + 8 * e) * kValueRow + b * 64));
+                        const u32x2 two = bits<u32x2>(four);
+                        words[2 * e] = two[0], words[2 * e + 1] = two[1];
+                    }
+#pragma unroll
+                    for (int term = 0; term < kTerms; ++term)
+                        sum[b] = Matrix<T>::mul32(bits<Vec>(words), p[t][term], sum[b]);
+                }
+            const uint64_t odd_tokens = uint64_t(odd[turn][1]) << 32 | odd[turn][0];
+            if (odd_tokens) {
+                for (uint64_t left = odd_tokens; left; left &= left - 1) {
+                    const int at = __builtin_ctzll(left);
+                    float weight = 0;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            weight = 32 * h + 8 * (i >> 2) + 4 * half + (i & 3) == at ? score[h][i] : weight;
+                    weight = sum_across_halves(weight);
+                    const int seen = token + at;
+                    const uint32_t page = a.block_size.divide(seen);
+                    const int block = table[page];
+                    const char* const value = values + (block * a.layer.block_stride +
+                                                        (seen - page * a.block_size.d) * a.layer.token_stride) * kBytes;
+                    float scale = 1;
+                    if constexpr (kEight)
+                        scale = power_of(scales[block * a.layer.scale_block_stride + a.layer.scale_side_stride]);
+                    const bool sees = seen <= position && seen > after;
+#pragma unroll
+                    for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const int d = 32 * b + 8 * (i >> 2) + 4 * half + (i & 3);
+                            if (d >= width || !sees) continue;
+                            float x;
+                            if constexpr (kEight)
+                                x = __builtin_amdgcn_cvt_f32_fp8(static_cast<uint8_t>(value[d]), 0) * scale;
+                            else x = static_cast<float>(reinterpret_cast<const T*>(value)[d]);
+                            if (!(__builtin_fabsf(x) < __builtin_inff())) sum[b][i] += weight * x;
+                        }
+                }
+            }
+        }
+
+        if (more) {
+            store(next, stage + kStage - now, is_ragged(token + kTileTokens), odd[turn_next]);
+            valid = __ballot(next.at != kNowhere);
+            next = after_next;
+        }
+        __syncthreads();
+        now = kStage - now;
+        turn = turn_next;
+    }
+
+    total = sum_across_halves(total);
+    if (!real) return;
+    const int64_t index = row * a.heads + head;
+    const float share = parts > 1 ? 1.0f : over(total);
+    float* const sums = parts > 1 ? part_sums(a, index, part) : nullptr;
+    Q* const out = static_cast<Q*>(a.out) + row * a.out_token_stride + head * a.out_head_stride;
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int d = 32 * b + 8 * i + 4 * half;
+            if (d >= width) continue;
+            if (parts > 1) {
+                *reinterpret_cast<f32x4*>(sums + d) = f32x4{sum[b][4 * i], sum[b][4 * i + 1], sum[b][4 * i + 2],
+                                                           sum[b][4 * i + 3]};
+            } else {
+                typedef Q Four __attribute__((ext_vector_type(4)));
+                Four four;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) four[k] = static_cast<Q>(sum[b][4 * i + k] * share);
+                *reinterpret_cast<Four*>(out + d) = four;
+            }
+        }
+    if (half == 0) {
+        if (parts > 1) {
+            float* const about = part_totals(a, index, part);
+            about[0] = top;
+            about[1] = total;
+        } else if (a.lse) {
+            a.lse[index] = top * a.scale + __builtin_logf(total);
+        }
+    }
+}
+
+// ----------------------------------------------------------------- parts joined
+
+// The parts of a row's head: a workgroup's threads take values along the row.
 template <typename Q>
 __global__ __launch_bounds__(256) void join_kernel(Attend a) {
     const int head = blockIdx.x % a.heads, row = blockIdx.x / a.heads;
-    const Sight sight = sight_of(a, row);
-    if (sight.sequence < 0) return;
-    const int parts = parts_of(a, sight);
-    if (parts < 2) return;                                  // the row's own workgroup wrote it
+    int sequence = row;
+    if (a.q.query_starts)
+        sequence = find_sequence(a.q.n_seqs, row, [&](int s) { return int64_t(a.q.query_starts[s]); });
+    const Rows rows = rows_of(a.q, sequence, a.tokens);
+    const int mine = row - rows.first;
+    if (mine < 0 || mine >= rows.count) return;             // padding
+    int parts;
+    if (rows.count == 1) {
+        parts = parts_of<kTile>(a.rows, sight_of(a, sequence, rows, 0, 0));
+    } else {
+        const int pair = mine * a.group + head % a.group;
+        parts = parts_of<kTileTokens>(a.tiles, tile_sight(a, sequence, rows, pair / kTileRows * kTileRows));
+    }
+    if (parts < 2) return;                                  // written by the one workgroup that took it
     const int width = a.layer.width;
     const int64_t index = int64_t(row) * a.heads + head;
-    const float* const from = a.part + index * a.chunks * width;
-    const float* const about = a.part + int64_t(a.tokens) * a.heads * a.chunks * width + index * a.chunks * 2;
+    const float* const from = part_sums(a, index, 0);
+    const float* const about = part_totals(a, index, 0);
     const float factor = a.scale * kLog2e;
     float most = -__builtin_inff();
     for (int c = 0; c < parts; ++c) most = __builtin_fmaxf(most, about[2 * c]);
     for (int d = threadIdx.x; d < width; d += 256) {
         float x = 0, all = 0;
         for (int c = 0; c < parts; ++c) {
-            const float mine = about[2 * c];
-            const float share = mine == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((mine - most) * factor);
+            const float mine_of = about[2 * c];
+            const float share = mine_of == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((mine_of - most) * factor);
             x += from[c * width + d] * share;
             all += about[2 * c + 1] * share;
         }
-        const float over = all > 0 ? 1.0f / all : all == 0 ? 0.0f : all;
-        static_cast<Q*>(a.out)[row * a.out_token_stride + head * a.out_head_stride + d] = static_cast<Q>(x * over);
+        static_cast<Q*>(a.out)[row * a.out_token_stride + head * a.out_head_stride + d] = static_cast<Q>(x * over(all));
         if (a.lse && d == 0) a.lse[index] = most * a.scale + __builtin_logf(all);
     }
 }
 
 // ----------------------------------------------------------------- launches
 
-// Tokens of a part, and parts of the longest row.
-struct Split {
-    int chunk, chunks;
-};
-
-Split split_of(int64_t jobs, int64_t longest) {
-    constexpr int64_t least = 4 * kTile * kWaves, wanted = 2048;
+// A row's tokens in parts, so that `jobs` rows fill the chip.
+Split split_rows(int64_t jobs, int64_t longest) {
+    constexpr int64_t step = kTile * kWaves, least = 4 * step, wanted = 2048;
     longest = std::max<int64_t>(longest, 1);
     int64_t chunk = std::max(least, longest * jobs / wanted);
-    chunk = (chunk + kTile * kWaves - 1) / (kTile * kWaves) * (kTile * kWaves);
-    return Split{static_cast<int>(std::min<int64_t>(chunk, 1 << 30)),
-                 static_cast<int>((longest + kTile - 1 + chunk - 1) / chunk)};
+    chunk = std::min<int64_t>((chunk + step - 1) / step * step, 1 << 29);
+    return Split{static_cast<int>(chunk), static_cast<int>((longest + kTile - 1 + chunk - 1) / chunk)};
 }
 
-// The tokens that a row may see, at most.
-int64_t longest_sight(int64_t max_length, int64_t window) {
-    return window > 0 ? std::min(window, max_length) : max_length;
+// The same for tiles of rows: whole where there are tiles for two workgroups a CU.
+Split split_tiles(int64_t jobs, int64_t longest) {
+    constexpr int64_t least = 8 * kTileTokens, wanted = 1024;
+    longest = std::max<int64_t>(longest, 1);
+    if (jobs >= wanted / 2) return Split{1 << 29, 1};
+    int64_t chunk = std::max(least, longest * jobs / wanted);
+    chunk = std::min<int64_t>((chunk + kTileTokens - 1) / kTileTokens * kTileTokens, 1 << 29);
+    return Split{static_cast<int>(chunk), static_cast<int>((longest + kTileTokens - 1 + chunk - 1) / chunk)};
+}
+
+struct Plan {
+    Split rows, tiles;
+    int parts;
+    int64_t tile_slots;
+};
+
+Plan plan_of(int64_t tokens, int n_seqs, bool ragged, int heads, int kv_heads, int64_t max_length, int64_t window) {
+    const int64_t longest = window > 0 ? std::min(window, max_length) : max_length;
+    const int64_t group = heads / kv_heads, head_tiles = (group + kHeadTile - 1) / kHeadTile;
+    Plan plan{};
+    plan.rows = split_rows(n_seqs * head_tiles * kv_heads, longest);
+    plan.parts = plan.rows.chunks;
+    if (ragged) {
+        plan.tile_slots = tokens * group / kTileRows + n_seqs;
+        // A tile's rows see from the first's window to the last's own token.
+        plan.tiles = split_tiles(plan.tile_slots * kv_heads,
+                                 std::min(max_length, longest + (kTileRows + group - 1) / group));
+        plan.parts = std::max(plan.parts, plan.tiles.chunks);
+    }
+    return plan;
+}
+
+size_t bytes_of(const Plan& plan, int64_t tokens, int heads, int width) {
+    return plan.parts < 2 ? 0 : static_cast<size_t>(tokens) * heads * plan.parts * (width + 2) * sizeof(float);
 }
 
 template <typename Q, bool kEight, int kJ>
@@ -525,16 +951,37 @@ void launch_rows(const Attend& a, unsigned grid, unsigned lds, hipStream_t strea
     else launch_rows_of<Q, kEight, 16>(a, grid, lds, stream);
 }
 
+template <typename Q, bool kEight>
+void launch_tiles(const Attend& a, unsigned grid, hipStream_t stream) {
+    const auto kernel = a.layer.width <= 64    ? attend_tile_kernel<Q, kEight, 64>
+                        : a.layer.width <= 96  ? attend_tile_kernel<Q, kEight, 96>
+                        : a.layer.width <= 128 ? attend_tile_kernel<Q, kEight, 128>
+                        : a.layer.width <= 192 ? attend_tile_kernel<Q, kEight, 192>
+                                               : attend_tile_kernel<Q, kEight, 256>;
+    hipLaunchKernelGGL(kernel, dim3(grid), dim3(kTileWaves * 64), 0, stream, a);
+}
+
+unsigned checked_grid(int64_t groups) {
+    require(groups < (int64_t(1) << 31), "attend: too many rows for one launch");
+    return static_cast<unsigned>(groups);
+}
+
 template <typename Q>
-void launch_attend(const Attend& a, hipStream_t stream) {
-    const int64_t grid = int64_t(a.tokens) * a.chunks * a.head_tiles * a.layer.kv_heads;
-    require(grid < (int64_t(1) << 31), "attend: too many rows for one launch");
+void launch_attend(const Attend& a, const Plan& plan, hipStream_t stream) {
+    const bool eight = a.layer.type == KVSNAP_E4M3;
+    if (plan.tile_slots) {
+        const unsigned grid = checked_grid(plan.tile_slots * a.tiles.chunks * a.layer.kv_heads);
+        if (eight) launch_tiles<Q, true>(a, grid, stream);
+        else launch_tiles<Q, false>(a, grid, stream);
+        check_launched("attend's tiles");
+    }
+    const unsigned grid = checked_grid(int64_t(a.q.n_seqs) * a.rows.chunks * a.head_tiles * a.layer.kv_heads);
     const unsigned lds = 4u * (kWaves * std::min(kHeadTile, a.group) * a.layer.width + 2 * kWaves * kHeadTile);
-    if (a.layer.type == KVSNAP_E4M3) launch_rows<Q, true>(a, static_cast<unsigned>(grid), lds, stream);
-    else launch_rows<Q, false>(a, static_cast<unsigned>(grid), lds, stream);
+    if (eight) launch_rows<Q, true>(a, grid, lds, stream);
+    else launch_rows<Q, false>(a, grid, lds, stream);
     check_launched("attend");
-    if (a.chunks > 1) {
-        hipLaunchKernelGGL(join_kernel<Q>, dim3(static_cast<unsigned>(a.tokens) * a.heads), dim3(256), 0, stream, a);
+    if (a.parts > 1) {
+        hipLaunchKernelGGL(join_kernel<Q>, dim3(checked_grid(int64_t(a.tokens) * a.heads)), dim3(256), 0, stream, a);
         check_launched("attend's join");
     }
 }
@@ -543,13 +990,10 @@ void launch_attend(const Attend& a, hipStream_t stream) {
 
 extern "C" {
 
-size_t kvsnap_attend_workspace_bytes(int64_t tokens, int n_seqs, int heads, int kv_heads, int width,
+size_t kvsnap_attend_workspace_bytes(int64_t tokens, int n_seqs, int ragged, int heads, int kv_heads, int width,
                                      int64_t max_length, int64_t window) {
-    (void)n_seqs;
-    if (tokens <= 0 || heads <= 0 || kv_heads <= 0) return 0;
-    const int64_t tiles = (heads / kv_heads + kHeadTile - 1) / kHeadTile;
-    const Split split = split_of(tokens * kv_heads * tiles, longest_sight(max_length, window));
-    return split.chunks < 2 ? 0 : static_cast<size_t>(tokens) * heads * split.chunks * (width + 2) * sizeof(float);
+    if (tokens <= 0 || n_seqs <= 0 || heads <= 0 || kv_heads <= 0) return 0;
+    return bytes_of(plan_of(tokens, n_seqs, ragged, heads, kv_heads, max_length, window), tokens, heads, width);
 }
 
 int kvsnap_attend(const kvsnap_paged_layer* layer, const kvsnap_sequences* sequences, const void* query,
@@ -565,6 +1009,7 @@ int kvsnap_attend(const kvsnap_paged_layer* layer, const kvsnap_sequences* seque
         require(scale > 0 && scale < 1e30f, "attend: the scale must be positive and finite");
         if (tokens == 0 || heads == 0 || sequences->n_seqs == 0) return;
         require(heads % layer->kv_heads == 0, "attend: query heads must be a multiple of the cache's");
+        require(tokens * heads < (int64_t(1) << 31), "attend: too many rows for one launch");
         require(sequences->query_starts || tokens == sequences->n_seqs,
                 "attend: without query_starts every sequence has one row");
         require(type == KVSNAP_BF16 || type == KVSNAP_FP16, "attend: queries must be bf16 or fp16");
@@ -584,21 +1029,20 @@ int kvsnap_attend(const kvsnap_paged_layer* layer, const kvsnap_sequences* seque
         a.out_token_stride = out_token_stride, a.out_head_stride = out_head_stride;
         a.tokens = static_cast<int>(tokens), a.heads = heads, a.group = heads / layer->kv_heads;
         a.scale = scale;
-        a.window = static_cast<int>(std::min<int64_t>(window, (int64_t(1) << 31) - 1));
+        a.window = static_cast<int>(std::min<int64_t>(window, 1 << 30));
         a.head_tiles = (a.group + kHeadTile - 1) / kHeadTile;
         a.block_size = Divider::of(layer->block_size);
+        a.group_size = Divider::of(a.group);
         const int64_t named = int64_t(sequences->table_width) * layer->block_size;
-        const Split split = split_of(tokens * layer->kv_heads * a.head_tiles,
-                                     longest_sight(std::min(max_length, named), window));
-        a.chunk = split.chunk, a.chunks = split.chunks;
+        const Plan plan = plan_of(tokens, sequences->n_seqs, sequences->query_starts != nullptr, heads,
+                                  layer->kv_heads, std::min(max_length, named), a.window);
+        a.rows = plan.rows, a.tiles = plan.tiles, a.parts = plan.parts;
         a.part = static_cast<float*>(workspace);
-        require(workspace_bytes >= kvsnap_attend_workspace_bytes(tokens, sequences->n_seqs, heads, layer->kv_heads,
-                                                                 layer->width, std::min(max_length, named), window),
-                "attend: the workspace is too small");
-        require(a.chunks < 2 || (workspace && reinterpret_cast<uintptr_t>(workspace) % 16 == 0),
+        require(workspace_bytes >= bytes_of(plan, tokens, heads, layer->width), "attend: the workspace is too small");
+        require(a.parts < 2 || (workspace && reinterpret_cast<uintptr_t>(workspace) % 16 == 0),
                 "attend: the workspace must be 16-byte aligned device memory");
         const auto launch = type == KVSNAP_BF16 ? launch_attend<__bf16> : launch_attend<_Float16>;
-        launch(a, reinterpret_cast<hipStream_t>(stream));
+        launch(a, plan, reinterpret_cast<hipStream_t>(stream));
     });
 }
 

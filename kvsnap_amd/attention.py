@@ -14,23 +14,20 @@ outputs and workspace (from torch's allocator, on the current stream), or keeps 
 them may be captured in a graph and replayed over changed tables.  Launches go to the current stream of the cache's
 device.  There is no CPU fallback: without the HIP library every call raises.
 
-The kernels' contract is in ``include/kvsnap_attention.h``.
+The kernels' contract is in ``include/kvsnap_attention.h``; arguments are checked in ``csrc/binding.cpp``.  No
+gradient is recorded: a tensor that requires one is refused outside ``torch.no_grad()``.
 """
 from __future__ import annotations
 
 import ctypes as C
-from functools import lru_cache
-import struct
 
 from .layout import describe_layer
-from .native import check as _check, kernel_library
+from .native import attention_binding
 
 __all__ = ["PagedCache", "block_scales", "rotary_table", "rotate"]
 
 #: Type codes of include/kvsnap_attention.h by torch type name.
-_TYPES = {"torch.bfloat16": 0, "torch.float16": 1, "torch.float8_e4m3fn": 2, "torch.float32": 3}
-_SEQUENCES = struct.Struct("=QQQqii").pack
-_ROTATION = struct.Struct("=QQqqiiii32s").pack
+_TYPES = {"torch.bfloat16": 0, "torch.float16": 1, "torch.float8_e4m3fn": 2}
 
 
 class _Layer(C.Structure):
@@ -61,78 +58,6 @@ def block_scales(blocks, layers, heads, *, device=None):
     return rows, [rows[:, at:at + 2 * heads].unflatten(1, (heads, 2)) for at in range(0, used, 2 * heads)]
 
 
-@lru_cache(maxsize=64)
-def _packed_axes(axes):
-    """Two bits a pair, 16 words of eight pairs."""
-    words = [0] * 16
-    for pair, axis in enumerate(axes):
-        words[pair // 8] |= axis << (2 * (pair % 8))
-    return struct.pack("=16H", *words)
-
-
-_ONE_AXIS = bytes(32)
-
-
-def _on_gpu(device, *tensors):
-    """The caller's device must be one GPU for all of a call's tensors (checked last: everything else can be found
-    wrong without one)."""
-    if device.type != "cuda" or any(t.device != device for t in tensors):
-        raise ValueError("every tensor of a call must be on one and the same CUDA device")
-
-
-def _rows(what, tensor, tokens, heads, width):
-    """A ``[tokens, heads, width]`` tensor (None: any) whose last axis is contiguous."""
-    if tensor.ndim != 3 or any(want is not None and have != want
-                               for have, want in zip(tensor.shape, (tokens, heads, width))):
-        want = ", ".join("any" if n is None else str(n) for n in (tokens, heads, width))
-        raise ValueError(f"{what} must be [{want}], not {list(tensor.shape)}")
-    if tensor.stride(2) != 1 and tensor.shape[2] > 1:
-        raise ValueError(f"{what}: the last axis must be contiguous")
-
-
-def _rotation(rotary, positions, tokens, width, axes, interleaved, inverse):
-    """The kernels' description of a rotation, and the tensors it reads; None without one."""
-    if rotary is None:
-        if positions is not None or axes is not None:
-            raise ValueError("positions and axes need a rotary table")
-        return None, ()
-    if rotary.ndim != 3 or rotary.shape[2] != 2 or str(rotary.dtype) != "torch.float32" or not rotary.is_contiguous():
-        raise ValueError("a rotary table is a contiguous float32 [positions, pairs, 2] tensor")
-    rows, pairs, _ = rotary.shape
-    if not pairs or pairs % 8 or 2 * pairs > width:
-        raise ValueError(f"a rotary table's pairs must be a multiple of 8 and at most {width // 2}, not {pairs}")
-    count, pointer, stride, narrow, tensors = 1, 0, 0, 0, (rotary,)
-    if positions is not None:
-        dtype = str(positions.dtype)
-        if dtype not in ("torch.int64", "torch.int32"):
-            raise ValueError("positions must be int64 or int32")
-        if positions.ndim not in (1, 2) or positions.shape[-1] != tokens or (
-                positions.stride(-1) != 1 and tokens > 1):
-            raise ValueError(f"positions must be [{tokens}] or [axes, {tokens}], the last axis contiguous")
-        if positions.ndim == 2:
-            count, stride = positions.shape[0], positions.stride(0)
-        pointer, narrow, tensors = positions.data_ptr(), dtype == "torch.int32", (rotary, positions)
-    packed = _ONE_AXIS
-    if axes is not None:
-        axes = tuple(axes)
-        if len(axes) != pairs or not 1 <= count <= 4 or not set(axes) <= set(range(count)):
-            raise ValueError(f"axes must name, for each of {pairs} pairs, one of the positions' {count} axes (4 at most)")
-        packed = _packed_axes(axes)
-    elif count != 1:
-        raise ValueError("positions of several axes need axes: the axis of each pair")
-    return _ROTATION(rotary.data_ptr(), pointer, rows, stride, pairs, bool(interleaved), narrow, bool(inverse),
-                     packed), tensors
-
-
-def _launch(device, launch):
-    """``launch(stream handle)`` with ``device`` current (the calling thread may have another)."""
-    import torch
-    if torch.cuda.current_device() == device.index:
-        return launch(torch.cuda.current_stream(device).cuda_stream)
-    with torch.cuda.device(device):
-        return launch(torch.cuda.current_stream(device).cuda_stream)
-
-
 def rotate(x, positions, rotary, *, axes=None, interleaved=False, inverse=False, out=None):
     """``x`` ([tokens, heads, width], bf16, fp16 or fp32) with each pair of a head's values turned by the angle of its
     token's position: (a, b) becomes (a cos - b sin, b cos + a sin), in fp32 and rounded once.
@@ -143,29 +68,7 @@ def rotate(x, positions, rotary, *, axes=None, interleaved=False, inverse=False,
     has no angle and gives NaN.  ``inverse`` turns the other way: it undoes a rotation, gives its gradient, and moves
     kept keys to earlier positions.  ``out`` (a new tensor if None) may be ``x`` itself.
     """
-    import torch
-    _rows("x", x, None, None, None)
-    tokens, heads, width = x.shape
-    kind = _TYPES.get(str(x.dtype), 2)
-    if kind == 2:
-        raise ValueError("x must be bfloat16, float16 or float32")
-    if width % 16 or not 0 < width <= 256:
-        raise ValueError(f"x's width must be a multiple of 16 up to 256, not {width}")
-    if positions is None or rotary is None:
-        raise ValueError("a rotation needs positions and a rotary table")
-    rotation, tensors = _rotation(rotary, positions, tokens, width, axes, interleaved, inverse)
-    if out is None:
-        out = torch.empty((tokens, heads, width), dtype=x.dtype, device=x.device)
-    else:
-        _rows("out", out, tokens, heads, width)
-        if out.dtype != x.dtype:
-            raise ValueError("out must have x's type")
-    _on_gpu(x.device, out, *tensors)
-    lib = kernel_library()
-    _launch(x.device, lambda stream: _check(lib, lib.kvsnap_rotate(
-        x.data_ptr(), x.stride(0), x.stride(1), out.data_ptr(), out.stride(0), out.stride(1), tokens, heads, width,
-        kind, rotation, stream)))
-    return out
+    return attention_binding().rotate(x, positions, rotary, axes, interleaved, inverse, out)
 
 
 class PagedCache:
@@ -222,26 +125,7 @@ class PagedCache:
         self._layer = _Layer(address, address + apart * size, scales.data_ptr() if scales is not None else None,
                              *strides, *scale_strides, blocks, block_size, heads, width, kind)
         self._layer_at = C.addressof(self._layer)
-
-    def _sequences(self, tokens, block_tables, lengths, query_starts):
-        """The kernels' description of the step's tables, and the tables."""
-        if block_tables.ndim != 2 or lengths.ndim != 1 or block_tables.shape[0] != lengths.shape[0]:
-            raise ValueError(f"block_tables must be [sequences, blocks] and lengths [sequences], not "
-                             f"{list(block_tables.shape)} and {list(lengths.shape)}")
-        tables = (block_tables, lengths) if query_starts is None else (block_tables, lengths, query_starts)
-        if any(str(t.dtype) != "torch.int32" for t in tables):
-            raise ValueError("block_tables, lengths and query_starts must be int32")
-        if any(t.stride(-1) != 1 and t.shape[-1] > 1 for t in tables):
-            raise ValueError("block_tables, lengths and query_starts must be contiguous along their last axis")
-        count, wide = block_tables.shape
-        if query_starts is None:
-            if tokens != count:
-                raise ValueError(f"{tokens} rows for {count} sequences of one row each: query_starts is needed")
-        elif query_starts.ndim != 1 or query_starts.shape[0] != count + 1:
-            raise ValueError(f"query_starts must be [{count + 1}], not {list(query_starts.shape)}")
-        return _SEQUENCES(block_tables.data_ptr(), lengths.data_ptr(),
-                          0 if query_starts is None else query_starts.data_ptr(), block_tables.stride(0), wide,
-                          count), tables
+        self._call = attention_binding()
 
     def append(self, key, value, block_tables, lengths, *, query_starts=None, query=None, positions=None, rotary=None,
                axes=None, interleaved=False, query_out=None):
@@ -256,41 +140,8 @@ class PagedCache:
         are not finite are stored as NaN.  Slots past the length stay as they are, and so do the rows of
         ``query_out`` that are padding.  Sequences of one call must not share a block that it writes.
         """
-        import torch
-        _rows("key", key, None, self.heads, self.width)
-        tokens = key.shape[0]
-        _rows("value", value, tokens, self.heads, self.width)
-        dtype = key.dtype
-        kind = _TYPES.get(str(dtype))
-        if kind not in (0, 1) or value.dtype != dtype or (self._kind != 2 and kind != self._kind):
-            raise ValueError(f"keys and values must both be bfloat16 or float16, a 16-bit cache's own type: "
-                             f"{key.dtype} and {value.dtype} into {self.cache.dtype}")
-        sequences, tensors = self._sequences(tokens, block_tables, lengths, query_starts)
-        rotation, more = _rotation(rotary, positions, tokens, self.width, axes, interleaved, False)
-        heads, rows = 0, (0, 0, 0)
-        out = (0, 0, 0)
-        if query is not None:
-            _rows("query", query, tokens, None, self.width)
-            if query.dtype != dtype:
-                raise ValueError("query must have the keys' type")
-            heads = query.shape[1]
-            if query_out is None:
-                query_out = torch.empty(query.shape, dtype=dtype, device=query.device)
-            else:
-                _rows("query_out", query_out, tokens, heads, self.width)
-                if query_out.dtype != dtype:
-                    raise ValueError("query_out must have the query's type")
-            rows = query.data_ptr(), query.stride(0), query.stride(1)
-            out = query_out.data_ptr(), query_out.stride(0), query_out.stride(1)
-            tensors = (*tensors, query, query_out)
-        elif query_out is not None:
-            raise ValueError("query_out needs a query")
-        _on_gpu(self.device, key, value, *tensors, *more)
-        lib = kernel_library()
-        _launch(self.device, lambda stream: _check(lib, lib.kvsnap_append(
-            self._layer_at, sequences, rotation, key.data_ptr(), key.stride(0), key.stride(1), value.data_ptr(),
-            value.stride(0), value.stride(1), *rows, *out, tokens, heads, kind, stream)))
-        return query_out
+        return self._call.append(self._layer_at, self.cache, key, value, block_tables, lengths, query_starts, query,
+                                 positions, rotary, axes, interleaved, query_out)
 
     def attend(self, query, block_tables, lengths, *, query_starts=None, max_length=None, softmax_scale=None,
                window=None, out=None, return_lse=False):
@@ -308,47 +159,5 @@ class PagedCache:
         logarithms of the rows' sums of exponentials (-inf for a row that sees nothing), by which attention over
         parts of the tokens can be joined.
         """
-        import torch
-        _rows("query", query, None, None, self.width)
-        tokens, heads, _ = query.shape
-        dtype = query.dtype
-        kind = _TYPES.get(str(dtype))
-        if kind not in (0, 1) or (self._kind != 2 and kind != self._kind):
-            raise ValueError(f"queries must be bfloat16 or float16, a 16-bit cache's own type: {dtype} over "
-                             f"{self.cache.dtype}")
-        if heads % self.heads or not heads:
-            raise ValueError(f"{heads} query heads do not share the cache's {self.heads}")
-        if window is not None and window < 1:
-            raise ValueError("a window holds at least the row's own token")
-        scale = self.width ** -0.5 if softmax_scale is None else softmax_scale
-        if not 0 < scale < 1e30:
-            raise ValueError("softmax_scale must be positive and finite")
-        sequences, tensors = self._sequences(tokens, block_tables, lengths, query_starts)
-        named = block_tables.shape[1] * self.block_size
-        if max_length is None or max_length > named:
-            max_length = named
-        elif max_length < 0:
-            raise ValueError("max_length must not be negative")
-        if out is None:
-            out = torch.empty((tokens, heads, self.width), dtype=dtype, device=query.device)
-        else:
-            _rows("out", out, tokens, heads, self.width)
-            if out.dtype != dtype:
-                raise ValueError("out must have the query's type")
-        _on_gpu(self.device, query, out, *tensors)
-        lse = torch.empty((tokens, heads), dtype=torch.float32, device=self.device) if return_lse else None
-        lib = kernel_library()
-        window = min(window or 0, 1 << 30)
-        size = _workspace_bytes(lib, tokens, block_tables.shape[0], query_starts is not None, heads, self.heads,
-                                self.width, max_length, window)
-        scratch = torch.empty(size, dtype=torch.uint8, device=self.device) if size else None
-        _launch(self.device, lambda stream: _check(lib, lib.kvsnap_attend(
-            self._layer_at, sequences, query.data_ptr(), query.stride(0), query.stride(1), out.data_ptr(),
-            out.stride(0), out.stride(1), lse.data_ptr() if return_lse else None, tokens, heads, kind, scale, window,
-            max_length, scratch.data_ptr() if size else None, size, stream)))
-        return (out, lse) if return_lse else out
-
-
-@lru_cache(maxsize=256)
-def _workspace_bytes(lib, *sizes):
-    return lib.kvsnap_attend_workspace_bytes(*sizes)
+        return self._call.attend(self._layer_at, self.cache, query, block_tables, lengths, query_starts, max_length,
+                                 softmax_scale, window, out, return_lse)

@@ -4,14 +4,16 @@
 
 ``_native/libkvsnap_hip.so``  pinned pool + HIP kernels + host record hashes (hipcc, gfx950)
 ``_native/libkvsnap_io.so``   host CRC32C + pread/pwrite pool (g++)
+``_native/kvsnap_binding.so`` the attention operators' calls from Python, on torch's tensors (g++)
 
-Both always rebuild when asked; the loaders only use what is already built.
+All always rebuild when asked; the loaders only use what is already built.
 """
 from __future__ import annotations
 
 import os
 import shutil
 import subprocess
+import sysconfig
 from pathlib import Path
 
 PACKAGE = Path(__file__).resolve().parent
@@ -19,6 +21,7 @@ CSRC = PACKAGE / "csrc"
 NATIVE = PACKAGE / "_native"
 HIP_LIBRARY = NATIVE / "libkvsnap_hip.so"
 IO_LIBRARY = NATIVE / "libkvsnap_io.so"
+BINDING = NATIVE / "kvsnap_binding.so"
 
 ARCH = os.environ.get("KVSNAP_OFFLOAD_ARCH", "gfx950")
 
@@ -67,8 +70,24 @@ def build_io(target: Path = IO_LIBRARY) -> Path:
     return target
 
 
+def build_binding(target: Path = BINDING) -> Path:
+    import torch
+    from torch.utils import cpp_extension
+    tmp = _atomic_output(target)
+    headers = [flag for path in cpp_extension.include_paths() for flag in ("-isystem", path)]
+    rocm = Path(_hipcc()).resolve().parent.parent / "include"
+    # HIP's own headers ask a host compiler which platform it builds for.
+    _run(["g++", "-std=c++17", "-O2", "-fPIC", "-shared", "-Wall", "-Wextra", "-Werror", "-D__HIP_PLATFORM_AMD__",
+          "-DUSE_ROCM", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+          f"-I{sysconfig.get_path('include')}", "-isystem", str(rocm), *headers, "-o", str(tmp),
+          str(CSRC / "binding.cpp"), *(f"-L{path}" for path in cpp_extension.library_paths()),
+          "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_python"])
+    os.replace(tmp, target)
+    return target
+
+
 def build_all() -> list[Path]:
-    return [build_io(), build_hip()]
+    return [build_io(), build_hip(), build_binding()]
 
 
 if __name__ == "__main__":

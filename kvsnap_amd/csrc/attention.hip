@@ -125,6 +125,12 @@ struct Split {
     int chunk, chunks;
 };
 
+// Where parts leave a head's unnormalised out ([heads, parts, width]), and its largest score and total ([heads, parts,
+// 2]), for heads counted over rows.
+struct Parts {
+    float *sums, *totals;
+};
+
 struct Attend {
     kvsnap_paged_layer layer;
     kvsnap_sequences q;
@@ -136,10 +142,9 @@ struct Attend {
     float scale;
     int window;                // 0: none
     Split rows, tiles;         // of a row alone, and of a tile of rows
-    int parts;                 // the more of the two's: room in `part`
+    Parts row_parts, tile_parts;  // by sequence, and by row
     int head_tiles;            // of 16 heads, of a key head's
     Divider block_size, group_size;
-    float* part;               // [tokens, heads, parts, width] sums, then [tokens, heads, parts, 2] largest and sum
 };
 
 constexpr int kTile = 32;         // tokens a wave takes at a time
@@ -163,14 +168,6 @@ template <int kTokens>
 __device__ __forceinline__ int parts_of(const Split& split, const Sight& sight) {
     const int first = sight.low & ~(kTokens - 1);
     return sight.high <= sight.low ? 0 : min((sight.high - first + split.chunk - 1) / split.chunk, split.chunks);
-}
-
-// Where a part's sums of a row's head are, and its largest score and total.
-__device__ __forceinline__ float* part_sums(const Attend& a, int64_t row_head, int part) {
-    return a.part + (row_head * a.parts + part) * a.layer.width;
-}
-__device__ __forceinline__ float* part_totals(const Attend& a, int64_t row_head, int part) {
-    return a.part + int64_t(a.tokens) * a.heads * a.parts * a.layer.width + (row_head * a.parts + part) * 2;
 }
 
 // One wave's loads of a tile: K's rows for the first product and V's for the second.
@@ -464,23 +461,18 @@ __global__ __launch_bounds__(kWaves * 64) void attend_row_kernel(Attend a) {
             y += from[1] * share;
             all += totals[w * kHeadTile + head] * share;
         }
-        const int64_t index = int64_t(row) * a.heads + first_head + head;
         if (parts > 1) {
-            float* const to = part_sums(a, index, part) + d;
-            to[0] = x;
-            to[1] = y;
-            if (d == 0) {
-                float* const about = part_totals(a, index, part);
-                about[0] = most;
-                about[1] = all;
-            }
+            const int64_t at_part = (int64_t(sequence) * a.heads + first_head + head) * a.rows.chunks + part;
+            *reinterpret_cast<float2*>(a.row_parts.sums + at_part * width + d) = float2{x, y};
+            if (d == 0) *reinterpret_cast<float2*>(a.row_parts.totals + at_part * 2) = float2{most, all};
         } else {
             const float share = over(all);
             Q* const to = static_cast<Q*>(a.out) + row * a.out_token_stride +
                           (first_head + head) * a.out_head_stride + d;
             to[0] = static_cast<Q>(x * share);
             to[1] = static_cast<Q>(y * share);
-            if (a.lse && d == 0) a.lse[index] = most * a.scale + __builtin_logf(all);
+            if (a.lse && d == 0)
+                a.lse[int64_t(row) * a.heads + first_head + head] = most * a.scale + __builtin_logf(all);
         }
     }
 }
@@ -819,7 +811,8 @@ __global__ __launch_bounds__(kTileWaves * 64, kD <= 128 ? 2 : 1) void attend_til
     if (!real) return;
     const int64_t index = row * a.heads + head;
     const float share = parts > 1 ? 1.0f : over(total);
-    float* const sums = parts > 1 ? part_sums(a, index, part) : nullptr;
+    const int64_t at_part = index * a.tiles.chunks + part;
+    float* const sums = a.tile_parts.sums + at_part * width;
     Q* const out = static_cast<Q*>(a.out) + row * a.out_token_stride + head * a.out_head_stride;
 #pragma unroll
     for (int b = 0; b < kBlocks; ++b)
@@ -840,9 +833,7 @@ __global__ __launch_bounds__(kTileWaves * 64, kD <= 128 ? 2 : 1) void attend_til
         }
     if (half == 0) {
         if (parts > 1) {
-            float* const about = part_totals(a, index, part);
-            about[0] = top;
-            about[1] = total;
+            *reinterpret_cast<float2*>(a.tile_parts.totals + at_part * 2) = float2{top, total};
         } else if (a.lse) {
             a.lse[index] = top * a.scale + __builtin_logf(total);
         }
@@ -851,28 +842,34 @@ __global__ __launch_bounds__(kTileWaves * 64, kD <= 128 ? 2 : 1) void attend_til
 
 // ----------------------------------------------------------------- parts joined
 
-// The parts of a row's head: a workgroup's threads take values along the row.
+// The parts of a row's head: a workgroup's threads take values along the row.  The first `alone` workgroups take the
+// sequences of one row, the others the rows of tiles.
 template <typename Q>
-__global__ __launch_bounds__(256) void join_kernel(Attend a) {
-    const int head = blockIdx.x % a.heads, row = blockIdx.x / a.heads;
-    int sequence = row;
-    if (a.q.query_starts)
-        sequence = find_sequence(a.q.n_seqs, row, [&](int s) { return int64_t(a.q.query_starts[s]); });
+__global__ __launch_bounds__(256) void join_kernel(Attend a, uint32_t alone) {
+    const bool single = blockIdx.x < alone;
+    const uint32_t job = single ? blockIdx.x : blockIdx.x - alone;
+    const int head = job % a.heads;
+    int sequence = job / a.heads, row = job / a.heads;
+    if (!single) sequence = find_sequence(a.q.n_seqs, row, [&](int s) { return int64_t(a.q.query_starts[s]); });
     const Rows rows = rows_of(a.q, sequence, a.tokens);
+    if (single) row = rows.first;
     const int mine = row - rows.first;
-    if (mine < 0 || mine >= rows.count) return;             // padding
+    if (mine < 0 || mine >= rows.count || (rows.count == 1) != single) return;
+    const int width = a.layer.width;
+    const int64_t index = int64_t(row) * a.heads + head;
     int parts;
-    if (rows.count == 1) {
+    const float *from, *about;
+    if (single) {
         parts = parts_of<kTile>(a.rows, sight_of(a, sequence, rows, 0, 0));
+        const int64_t first = (int64_t(sequence) * a.heads + head) * a.rows.chunks;
+        from = a.row_parts.sums + first * width, about = a.row_parts.totals + first * 2;
     } else {
         const int pair = mine * a.group + head % a.group;
         parts = parts_of<kTileTokens>(a.tiles, tile_sight(a, sequence, rows, pair / kTileRows * kTileRows));
+        const int64_t first = index * a.tiles.chunks;
+        from = a.tile_parts.sums + first * width, about = a.tile_parts.totals + first * 2;
     }
     if (parts < 2) return;                                  // written by the one workgroup that took it
-    const int width = a.layer.width;
-    const int64_t index = int64_t(row) * a.heads + head;
-    const float* const from = part_sums(a, index, 0);
-    const float* const about = part_totals(a, index, 0);
     const float factor = a.scale * kLog2e;
     float most = -__builtin_inff();
     for (int c = 0; c < parts; ++c) most = __builtin_fmaxf(most, about[2 * c]);
@@ -912,8 +909,7 @@ Split split_tiles(int64_t jobs, int64_t longest) {
 
 struct Plan {
     Split rows, tiles;
-    int parts;
-    int64_t tile_slots;
+    int64_t tile_slots, row_parts, tile_parts;  // parts: of all heads, 0 where rows are whole
 };
 
 Plan plan_of(int64_t tokens, int n_seqs, bool ragged, int heads, int kv_heads, int64_t max_length, int64_t window) {
@@ -921,19 +917,19 @@ Plan plan_of(int64_t tokens, int n_seqs, bool ragged, int heads, int kv_heads, i
     const int64_t group = heads / kv_heads, head_tiles = (group + kHeadTile - 1) / kHeadTile;
     Plan plan{};
     plan.rows = split_rows(n_seqs * head_tiles * kv_heads, longest);
-    plan.parts = plan.rows.chunks;
+    plan.row_parts = plan.rows.chunks < 2 ? 0 : int64_t(n_seqs) * heads * plan.rows.chunks;
     if (ragged) {
         plan.tile_slots = tokens * group / kTileRows + n_seqs;
         // A tile's rows see from the first's window to the last's own token.
         plan.tiles = split_tiles(plan.tile_slots * kv_heads,
                                  std::min(max_length, longest + (kTileRows + group - 1) / group));
-        plan.parts = std::max(plan.parts, plan.tiles.chunks);
+        plan.tile_parts = plan.tiles.chunks < 2 ? 0 : tokens * heads * plan.tiles.chunks;
     }
     return plan;
 }
 
-size_t bytes_of(const Plan& plan, int64_t tokens, int heads, int width) {
-    return plan.parts < 2 ? 0 : static_cast<size_t>(tokens) * heads * plan.parts * (width + 2) * sizeof(float);
+size_t bytes_of(const Plan& plan, int width) {
+    return static_cast<size_t>(plan.row_parts + plan.tile_parts) * (width + 2) * sizeof(float);
 }
 
 template <typename Q, bool kEight, int kJ>
@@ -980,8 +976,11 @@ void launch_attend(const Attend& a, const Plan& plan, hipStream_t stream) {
     if (eight) launch_rows<Q, true>(a, grid, lds, stream);
     else launch_rows<Q, false>(a, grid, lds, stream);
     check_launched("attend");
-    if (a.parts > 1) {
-        hipLaunchKernelGGL(join_kernel<Q>, dim3(checked_grid(int64_t(a.tokens) * a.heads)), dim3(256), 0, stream, a);
+    if (plan.row_parts + plan.tile_parts) {
+        const int64_t alone = plan.row_parts ? int64_t(a.q.n_seqs) * a.heads : 0;
+        const int64_t others = plan.tile_parts ? int64_t(a.tokens) * a.heads : 0;
+        hipLaunchKernelGGL(join_kernel<Q>, dim3(checked_grid(alone + others)), dim3(256), 0, stream, a,
+                           static_cast<uint32_t>(alone));
         check_launched("attend's join");
     }
 }
@@ -993,7 +992,7 @@ extern "C" {
 size_t kvsnap_attend_workspace_bytes(int64_t tokens, int n_seqs, int ragged, int heads, int kv_heads, int width,
                                      int64_t max_length, int64_t window) {
     if (tokens <= 0 || n_seqs <= 0 || heads <= 0 || kv_heads <= 0) return 0;
-    return bytes_of(plan_of(tokens, n_seqs, ragged, heads, kv_heads, max_length, window), tokens, heads, width);
+    return bytes_of(plan_of(tokens, n_seqs, ragged, heads, kv_heads, max_length, window), width);
 }
 
 int kvsnap_attend(const kvsnap_paged_layer* layer, const kvsnap_sequences* sequences, const void* query,
@@ -1036,10 +1035,13 @@ int kvsnap_attend(const kvsnap_paged_layer* layer, const kvsnap_sequences* seque
         const int64_t named = int64_t(sequences->table_width) * layer->block_size;
         const Plan plan = plan_of(tokens, sequences->n_seqs, sequences->query_starts != nullptr, heads,
                                   layer->kv_heads, std::min(max_length, named), a.window);
-        a.rows = plan.rows, a.tiles = plan.tiles, a.parts = plan.parts;
-        a.part = static_cast<float*>(workspace);
-        require(workspace_bytes >= bytes_of(plan, tokens, heads, layer->width), "attend: the workspace is too small");
-        require(a.parts < 2 || (workspace && reinterpret_cast<uintptr_t>(workspace) % 16 == 0),
+        a.rows = plan.rows, a.tiles = plan.tiles;
+        float* const room = static_cast<float*>(workspace);
+        const int64_t parts = plan.row_parts + plan.tile_parts;
+        a.row_parts = Parts{room, room + parts * layer->width};
+        a.tile_parts = Parts{room + plan.row_parts * layer->width, a.row_parts.totals + plan.row_parts * 2};
+        require(workspace_bytes >= bytes_of(plan, layer->width), "attend: the workspace is too small");
+        require(parts == 0 || (workspace && reinterpret_cast<uintptr_t>(workspace) % 16 == 0),
                 "attend: the workspace must be 16-byte aligned device memory");
         const auto launch = type == KVSNAP_BF16 ? launch_attend<__bf16> : launch_attend<_Float16>;
         launch(a, plan, reinterpret_cast<hipStream_t>(stream));

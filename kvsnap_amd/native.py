@@ -5,6 +5,7 @@
   12-25``, with its ``KVSNAP_CUDA_LIBRARY`` override first).
 * ``kernel_library`` loads it once per path, types every kernel entry point
   (``include/kvsnap_kernels.h``, ``include/kvsnap_attention.h``) and refuses another kernel ABI.
+* ``attention_binding`` loads the attention operators' calls over it.
 * ``HostStaging`` holds the small pinned buffers that launch tables cross the
   host link in (see its docstring for why torch's pinned copies are not used).
 
@@ -14,6 +15,8 @@ from __future__ import annotations
 
 import ctypes as C
 from contextlib import contextmanager
+from importlib.machinery import ExtensionFileLoader
+from importlib.util import module_from_spec, spec_from_file_location
 import os
 from pathlib import Path
 import threading
@@ -99,6 +102,28 @@ def kernel_library(library=None):
                 raise RuntimeError(f"unsupported kvsnap HIP kernel ABI {version}; rebuild the library")
             _loaded[key] = lib
     return lib
+
+
+_bound = None
+
+
+def attention_binding():
+    """The attention operators' calls (``_native/kvsnap_binding.so``), over the loaded HIP library's entry points;
+    raises if either is not built."""
+    global _bound
+    if _bound is None:
+        lib = kernel_library()
+        path = NATIVE / "kvsnap_binding.so"
+        if not path.is_file():
+            raise RuntimeError(f"attention binding not built ({path}); run python -m kvsnap_amd.build")
+        import torch  # noqa: F401  (the binding links against its libraries, loaded by now)
+        loader = ExtensionFileLoader("kvsnap_binding", str(path))
+        binding = module_from_spec(spec_from_file_location("kvsnap_binding", str(path), loader=loader))
+        loader.exec_module(binding)
+        binding.bind(*(C.cast(getattr(lib, name), C.c_void_p).value for name in (
+            "kvsnap_rotate", "kvsnap_append", "kvsnap_attend", "kvsnap_attend_workspace_bytes", "kvsnap_cuda_error")))
+        _bound = binding
+    return _bound
 
 
 def check(lib, rc):

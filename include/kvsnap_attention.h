@@ -103,10 +103,10 @@ int kvsnap_append(const kvsnap_paged_layer* layer, const kvsnap_sequences* seque
                   int64_t query_head_stride, void* query_out, int64_t out_token_stride, int64_t out_head_stride,
                   int64_t tokens, int heads, int type, uintptr_t stream);
 
-/* Device bytes of scratch that kvsnap_attend needs for these sizes (0: none);
+/* Device bytes of scratch that kvsnap_attend needs over this layer (0: none);
  * ragged: whether it is given query_starts.  A max_length above what the
  * tables name counts as that. */
-size_t kvsnap_attend_workspace_bytes(int64_t tokens, int n_seqs, int ragged, int heads, int kv_heads, int width,
+size_t kvsnap_attend_workspace_bytes(const kvsnap_paged_layer* layer, int64_t tokens, int n_seqs, int ragged, int heads,
                                      int64_t max_length, int64_t window);
 
 /* out[row, h] = the sum over the tokens t that a row sees of softmax(scale *

@@ -125,10 +125,15 @@ struct Split {
     int chunk, chunks;
 };
 
-// Where parts leave a head's unnormalised out ([heads, parts, width]), and its largest score and total ([heads, parts,
-// 2]), for heads counted over rows.
+// Where parts leave a head's unnormalised out, and its largest score and total.
 struct Parts {
     float *sums, *totals;
+};
+
+// Rows alone: how their tokens are cut into workgroups' jobs.
+struct RowJobs {
+    int even;      // cut into equal parts, by the lengths that the sequences have, or `chunks` of `chunk` tiles each
+    int chunk, chunks, wanted;   // even: at least `chunk` tiles, for about `wanted` jobs
 };
 
 struct Attend {
@@ -141,14 +146,18 @@ struct Attend {
     int tokens, heads, group;  // group: query heads that share a key head
     float scale;
     int window;                // 0: none
-    Split rows, tiles;         // of a row alone, and of a tile of rows
-    Parts row_parts, tile_parts;  // by sequence, and by row
+    RowJobs rows;
+    Split tiles;               // of a tile of rows
+    Parts row_parts, tile_parts;  // [job, beside, heads of a tile], and [row, head, part]
+    int2* row_info;               // [sequence, heads' group]: the first job and the parts of rows alone
     int head_tiles;            // of 16 heads, of a key head's
-    Divider block_size, group_size;
+    int beside;                // key heads that a workgroup's waves take side by side
+    int slots;                 // heads of a tile, at most
+    Divider block_size, group_size, all_heads, quarter_width;
 };
 
 constexpr int kTile = 32;         // tokens a wave takes at a time
-constexpr int kWaves = 4;         // of a workgroup, side by side along the tokens
+constexpr int kWaves = 8;         // of a workgroup
 constexpr int kHeadTile = 16;     // query rows of a product
 
 // What rows see, first to last: tokens [low, high) of their sequence, the first row at position `position`.
@@ -170,6 +179,70 @@ __device__ __forceinline__ int parts_of(const Split& split, const Sight& sight) 
     return sight.high <= sight.low ? 0 : min((sight.high - first + split.chunk - 1) / split.chunk, split.chunks);
 }
 
+// A job of the rows alone: a part of a sequence's tiles of tokens, for a workgroup's heads.
+struct RowJob {
+    int sequence, heads, part, parts, chunk;   // heads: which of the row's groups of heads; chunk: tiles of a part
+    int64_t first;                             // the sequence's first job; its parts' lie `head_groups` apart
+};
+
+// Tiles of tokens that a sequence's one row sees; 1 where it sees nothing, which is written too, and 0 for a sequence
+// of no or of more rows.
+__device__ __forceinline__ int row_tiles(const Attend& a, int sequence) {
+    const Rows rows = rows_of(a.q, sequence, a.tokens);
+    if (rows.count != 1) return 0;
+    const Sight sight = sight_of(a, sequence, rows, 0, 0);
+    return max((sight.high - (sight.low & ~(kTile - 1)) + kTile - 1) / kTile, 1);
+}
+
+__device__ __forceinline__ int wave_sum(int x) {
+#pragma unroll
+    for (int step = 1; step < 64; step <<= 1) x += __shfl_xor(x, step);
+    return __builtin_amdgcn_readfirstlane(x);
+}
+
+// Where even parts are cut: all sequences' tiles over the jobs wanted, in whole turns of a workgroup's waves.
+__device__ __forceinline__ int even_chunk(const Attend& a, int head_groups) {
+    const int lane = __lane_id(), in_turn = kWaves / a.beside;
+    int64_t all = 0;
+    for (int s = 0; s < a.q.n_seqs; s += 64) all += wave_sum(s + lane < a.q.n_seqs ? row_tiles(a, s + lane) : 0);
+    const int chunk = static_cast<int>(max(int64_t(a.rows.chunk), (all * head_groups + a.rows.wanted - 1) / a.rows.wanted));
+    return (chunk + in_turn - 1) / in_turn * in_turn;
+}
+
+// The sequence whose jobs hold `job`, and its parts.  A wave goes over 64 sequences at a time, their jobs summed from
+// the first on.
+__device__ __forceinline__ RowJob row_job(const Attend& a, int64_t job, int head_groups) {
+    if (!a.rows.even) {
+        const int sequence = static_cast<int>(job / (a.rows.chunks * head_groups));
+        const int64_t first = int64_t(sequence) * a.rows.chunks * head_groups;
+        const int rest = static_cast<int>(job - first), tiles = row_tiles(a, sequence);
+        // The last part that there is room for takes what is left.
+        return RowJob{tiles ? sequence : -1, rest % head_groups, rest / head_groups,
+                      min((tiles + a.rows.chunk - 1) / a.rows.chunk, a.rows.chunks), a.rows.chunk, first};
+    }
+    const int lane = __lane_id(), chunk = even_chunk(a, head_groups);
+    int64_t before = 0;
+    for (int s = 0; s < a.q.n_seqs; s += 64) {
+        const int mine = s + lane < a.q.n_seqs ? (row_tiles(a, s + lane) + chunk - 1) / chunk : 0;
+        int up_to = mine;
+#pragma unroll
+        for (int step = 1; step < 64; step <<= 1) {
+            const int other = __shfl_up(up_to, step);
+            up_to += lane >= step ? other : 0;
+        }
+        const uint64_t holds = __ballot(before + int64_t(up_to) * head_groups > job);
+        if (holds) {
+            const int at = __builtin_ctzll(holds);
+            const int parts = __builtin_amdgcn_readlane(mine, at);
+            const int64_t first = before + int64_t(__builtin_amdgcn_readlane(up_to, at) - parts) * head_groups;
+            const int rest = static_cast<int>(job - first);
+            return RowJob{parts ? s + at : -1, rest % head_groups, rest / head_groups, parts, chunk, first};
+        }
+        before += int64_t(__builtin_amdgcn_readlane(up_to, 63)) * head_groups;
+    }
+    return RowJob{-1, 0, 0, 0, 0, 0};
+}
+
 // One wave's loads of a tile: K's rows for the first product and V's for the second.
 template <bool kEight, int kJ>
 struct Tile {
@@ -185,8 +258,8 @@ struct Tile {
 //
 // Bound by reading K and V once: 16 query rows of a product are used for `group` heads, a quarter of them for groups
 // of four, and the matrix cores still wait for memory.
-template <typename Q, bool kEight, int kJ, bool kWhole>
-__global__ __launch_bounds__(kWaves * 64) void attend_row_kernel(Attend a) {
+template <typename Q, bool kEight, int kJ, bool kWhole, bool kExact>
+__global__ __launch_bounds__(kWaves * 64, kEight && kJ <= 8 ? 4 : 2) void attend_row_kernel(Attend a) {
     using T = typename Shape<Q, kEight>::T;
     using Vec = typename Matrix<T>::Vec;
     constexpr int kTerms = Shape<Q, kEight>::kTerms;
@@ -194,23 +267,22 @@ __global__ __launch_bounds__(kWaves * 64) void attend_row_kernel(Attend a) {
     using Loads = Tile<kEight, kJ>;
     constexpr int kRounds = Loads::kRounds, kWords = Loads::kWords, kBytes = Loads::kBytes;
 
-    const int kv_heads = a.layer.kv_heads;
-    uint32_t job = blockIdx.x;
-    const int kv_head = job % kv_heads;
-    job /= kv_heads;
-    const int head_tile = job % a.head_tiles;
-    job /= a.head_tiles;
-    const int part = job % a.rows.chunks, sequence = job / a.rows.chunks;
-    const Rows rows = rows_of(a.q, sequence, a.tokens);
-    if (rows.count != 1) return;                            // tiles take sequences of more rows
-    const int row = rows.first;
-    const Sight sight = sight_of(a, sequence, rows, 0, 0);
-    const int parts = parts_of<kTile>(a.rows, sight);
-    if (part >= max(parts, 1)) return;                      // the first part of a row that sees nothing writes zeros
-
-    const int width = a.layer.width, size = a.layer.block_size;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int column = lane & 15, quarter = lane >> 4;
+    // `beside` waves take key heads side by side, and those of one key head its tiles in turn.
+    const int beside = a.beside, in_turn = kWaves / beside, turn = wave / beside;
+    const int head_groups = a.layer.kv_heads / beside * a.head_tiles;
+    const RowJob job = row_job(a, blockIdx.x, head_groups);
+    if (job.sequence < 0 || job.part >= job.parts) return;
+    const int sequence = job.sequence, part = job.part, parts = job.parts;
+    if (a.row_info && part == 0 && threadIdx.x == 0)
+        a.row_info[int64_t(sequence) * head_groups + job.heads] = int2{static_cast<int>(job.first), parts};
+    const int kv_head = job.heads / a.head_tiles * beside + wave % beside, head_tile = job.heads % a.head_tiles;
+    const Rows rows = rows_of(a.q, sequence, a.tokens);
+    const int row = rows.first;
+    const Sight sight = sight_of(a, sequence, rows, 0, 0);
+
+    const int width = a.layer.width, size = a.layer.block_size;
     const int first_head = kv_head * a.group + head_tile * kHeadTile;
     const int heads = min(kHeadTile, a.group - head_tile * kHeadTile);
 
@@ -239,8 +311,8 @@ __global__ __launch_bounds__(kWaves * 64) void attend_row_kernel(Attend a) {
     float top = -__builtin_inff(), total = 0;
     const float factor = a.scale * kLog2e;
 
-    const int base = (sight.low & ~(kTile - 1)) + part * a.rows.chunk;
-    const int stop = part == a.rows.chunks - 1 ? sight.high : min(sight.high, base + a.rows.chunk);
+    const int base = (sight.low & ~(kTile - 1)) + part * job.chunk * kTile;
+    const int stop = part == parts - 1 ? sight.high : min(sight.high, base + job.chunk * kTile);
     const int32_t* const table = a.q.block_tables + sequence * a.q.table_stride;
     const char* const keys = static_cast<const char*>(a.layer.key) + kv_head * a.layer.head_stride * kBytes;
     const char* const values = static_cast<const char*>(a.layer.value) + kv_head * a.layer.head_stride * kBytes;
@@ -248,17 +320,28 @@ __global__ __launch_bounds__(kWaves * 64) void attend_row_kernel(Attend a) {
     const int row_bytes = static_cast<int>(a.layer.token_stride) * kBytes;
     const int64_t block_bytes = a.layer.block_stride * kBytes;
 
-    // Blocks of 16-token groups (kWhole: a block is whole groups): lane i holds that of group `cached` + i.
-    int cached = -64, block_of = -1;
-    float k_scale_of = 0, v_scale_of = 0;
     const auto block_at = [&](int token) -> int {           // of the table, -1 where there is none
         const uint32_t page = a.block_size.divide(token);
         if (page >= static_cast<uint32_t>(a.q.table_width) || token >= stop) return -1;
         const int block = table[page];
         return static_cast<uint32_t>(block) < static_cast<uint64_t>(a.layer.blocks) ? block : -1;
     };
+    // kWhole: lane i holds the block of the 16-token group `cached` + i, and its scales.
+    int cached = -64, block_of = -1;
+    float k_scale_of = 0, v_scale_of = 0;
+    const uint32_t k_lane = column * row_bytes + quarter * 16;
+    uint32_t v_lane[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        v_lane[i] = (quarter * 4 + i) * row_bytes + (column * kJ < width ? column * kJ * kBytes : 0);
 
-    const auto load_k = [&](Loads& tile, int token) {
+    // A tile's rows: 16 tokens by 16 lanes for K, four by a lane for V.  A block that the table does not name is read as
+    // block 0, and its tokens are masked.
+    Loads tile;
+    uint32_t mask = 0;          // bit 4 h + i: this lane's token 16 h + 4 quarter + i is seen
+    int64_t whole_offset[2];    // kWhole: where the tile's two groups of 16 tokens are
+    const auto load_k = [&](int token) {
+        mask = 0xff;
         if constexpr (kWhole) {
             const int group = token >> 4;
             if (group + 2 > cached + 64) {
@@ -270,84 +353,77 @@ __global__ __launch_bounds__(kWaves * 64) void attend_row_kernel(Attend a) {
                     v_scale_of = power_of(scale[a.layer.scale_side_stride]);
                 }
             }
-        }
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            int block, slot;
-            if constexpr (kWhole) {
+            for (int h = 0; h < 2; ++h) {
                 const int at = token + 16 * h;
-                block = __builtin_amdgcn_readlane(block_of, (at >> 4) - cached);
-                slot = at - a.block_size.divide(at) * size + column;
-                if constexpr (kEight)
-                    tile.k_scale[h] = bits<float>(
-                        __builtin_amdgcn_readlane(bits<int>(k_scale_of), (at >> 4) - cached));
-            } else {
-                const int at = token + 16 * h + column;
-                block = block_at(at);
-                slot = at - a.block_size.divide(at) * size;
-                if constexpr (kEight)
-                    tile.k_scale[h] = power_of(scales[max(block, 0) * a.layer.scale_block_stride]);
-            }
-            const char* const from = keys + block * block_bytes + slot * row_bytes;
+                const int block = __builtin_amdgcn_readlane(block_of, (at >> 4) - cached);
+                whole_offset[h] = max(block, 0) * block_bytes +
+                                  int64_t(at - a.block_size.divide(at) * size) * row_bytes;
+                if (block < 0) mask &= ~(0xfu << (4 * h));
 #pragma unroll
-            for (int r = 0; r < kRounds; ++r) {
-                const int at = (r * 4 + quarter) * 16;      // bytes of the row
-                tile.k[h][r] = u32x4{0, 0, 0, 0};
-                if (block >= 0 && at < width * kBytes) tile.k[h][r] = *reinterpret_cast<const u32x4*>(from + at);
-            }
-        }
-    };
-    const auto load_v = [&](Loads& tile, int token) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                int block, slot;
-                if constexpr (kWhole) {
-                    const int at = token + 16 * h;
-                    block = __builtin_amdgcn_readlane(block_of, (at >> 4) - cached);
-                    slot = at - a.block_size.divide(at) * size + quarter * 4 + i;
-                    if constexpr (kEight)
-                        tile.v_scale[h][i] = bits<float>(
-                            __builtin_amdgcn_readlane(bits<int>(v_scale_of), (at >> 4) - cached));
-                } else {
-                    const int at = token + 16 * h + quarter * 4 + i;
-                    block = block_at(at);
-                    slot = at - a.block_size.divide(at) * size;
-                    if constexpr (kEight)
-                        tile.v_scale[h][i] = power_of(
-                            scales[max(block, 0) * a.layer.scale_block_stride + a.layer.scale_side_stride]);
+                for (int r = 0; r < kRounds; ++r) {
+                    if (kExact || r * 64 + quarter * 16 < width * kBytes)
+                        tile.k[h][r] = *reinterpret_cast<const u32x4*>(keys + whole_offset[h] + k_lane + r * 64);
+                    else
+                        tile.k[h][r] = u32x4{0, 0, 0, 0};
                 }
-                const char* const from = values + block * block_bytes + slot * row_bytes + column * kJ * kBytes;
+            }
+        } else {
 #pragma unroll
-                for (int w = 0; w < kWords; ++w) tile.v[h][i][w] = 0;
-                if (block >= 0 && column * kJ < width) load_words<kWords>(from, tile.v[h][i]);
+            for (int h = 0; h < 2; ++h) {
+                const int at = token + 16 * h + column;
+                const int block = max(block_at(at), 0), slot = at - a.block_size.divide(at) * size;
+                const int64_t offset = block * block_bytes + int64_t(slot) * row_bytes;
+#pragma unroll
+                for (int r = 0; r < kRounds; ++r) {
+                    tile.k[h][r] = u32x4{0, 0, 0, 0};
+                    if (r * 64 + quarter * 16 < width * kBytes)
+                        tile.k[h][r] = *reinterpret_cast<const u32x4*>(keys + offset + r * 64 + quarter * 16);
+                }
+                if constexpr (kEight) tile.k_scale[h] = power_of(scales[block * a.layer.scale_block_stride]);
+            }
+        }
+        if (token < sight.low || token + kTile > stop) {
+#pragma unroll
+            for (int t = 0; t < 8; ++t) {
+                const int at = token + 16 * (t >> 2) + 4 * quarter + (t & 3);
+                if (at < sight.low || at >= stop) mask &= ~(1u << t);
             }
         }
     };
-
-    const auto visible = [&](int token) { return token >= sight.low && token < stop; };
-    // A token is seen if it is in sight and its block is one of the cache's.
-    const auto seen_mask = [&](int token) -> uint32_t {     // bit 4h + i: token + 16 h + 4 quarter + i
-        uint32_t mask = 0;
+    const auto load_v = [&](int token) {
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int at = token + 16 * h + 4 * quarter + i;
-                bool ok = visible(at);
-                if constexpr (kWhole) ok = ok && __builtin_amdgcn_readlane(block_of, ((token >> 4) + h) - cached) >= 0;
-                else ok = ok && block_at(at) >= 0;
-                mask |= ok ? 1u << (4 * h + i) : 0;
+                if constexpr (kWhole) {
+                    load_words<kWords>(values + whole_offset[h] + v_lane[i], tile.v[h][i]);
+                } else {
+                    const int at = token + 16 * h + quarter * 4 + i;
+                    const int named = block_at(at), block = max(named, 0);
+                    if (named < 0) mask &= ~(1u << (4 * h + i));
+                    const int64_t offset = block * block_bytes + int64_t(at - a.block_size.divide(at) * size) * row_bytes;
+                    load_words<kWords>(values + offset + v_lane[i] - (quarter * 4 + i) * row_bytes, tile.v[h][i]);
+                    if constexpr (kEight)
+                        tile.v_scale[h][i] =
+                            power_of(scales[block * a.layer.scale_block_stride + a.layer.scale_side_stride]);
+                }
             }
-        return mask;
+        if constexpr (kWhole && kEight) {       // behind the loads, which do not wait for them
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int at = (token >> 4) + h - cached;
+                tile.k_scale[h] = bits<float>(__builtin_amdgcn_readlane(bits<int>(k_scale_of), at));
+                tile.v_scale[h][0] = bits<float>(__builtin_amdgcn_readlane(bits<int>(v_scale_of), at));
+            }
+        }
     };
 
-    for (int token = base + wave * kTile; token < stop; token += kWaves * kTile) {
-        Loads tile;
-        load_k(tile, token);
-        load_v(tile, token);
-        const uint32_t mask = seen_mask(token);
+    for (int token = base + turn * kTile; token < stop; token += in_turn * kTile) {
+        load_k(token);
+        load_v(token);
+        const uint32_t seen = mask;
+        const bool ragged = __ballot(seen != 0xff) != 0;    // in most tiles every token is seen by every row
 
         f32x4 score[2];
 #pragma unroll
@@ -369,15 +445,14 @@ __global__ __launch_bounds__(kWaves * 64) void attend_row_kernel(Attend a) {
                 for (int t = 0; t < kTerms; ++t) score[h] = Matrix<T>::mul16(k, q[s][t], score[h]);
             }
         }
-
+        if (ragged) {
+#pragma unroll
+            for (int t = 0; t < 8; ++t)
+                score[t >> 2][t & 3] = seen >> t & 1 ? score[t >> 2][t & 3] : -__builtin_inff();
+        }
         float most = -__builtin_inff();
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                score[h][i] = mask >> (4 * h + i) & 1 ? score[h][i] : -__builtin_inff();
-                most = __builtin_fmaxf(most, score[h][i]);
-            }
+        for (int t = 0; t < 8; ++t) most = __builtin_fmaxf(most, score[t >> 2][t & 3]);
         most = max_across_groups(most);
         if (__ballot(most > top)) {
             const float grown = __builtin_fmaxf(top, most);
@@ -390,30 +465,33 @@ __global__ __launch_bounds__(kWaves * 64) void attend_row_kernel(Attend a) {
         const float against = top == -__builtin_inff() ? 0.0f : top * factor;
         Vec p[kTerms];
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(score[h][i], factor, -against));
-                total += x;
-                if constexpr (kTerms == 2) two_terms(x, p[0], p[1], 4 * h + i);
-                else p[0][4 * h + i] = static_cast<T>(x);
-            }
+        for (int t = 0; t < 8; ++t) {
+            const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(score[t >> 2][t & 3], factor, -against));
+            total += x;
+            if constexpr (kTerms == 2) two_terms(x, p[0], p[1], t);
+            else p[0][t] = static_cast<T>(x);
+        }
 
         // V^T: the tokens of this lane's column of values, from rows of values: pairs of 16-bit words change places.
         uint32_t wide[2][4][kJ / 2];
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const bool ok = mask >> (4 * h + i) & 1;    // what is not seen may hold anything: 0 * NaN is NaN
+            for (int i = 0; i < 4; ++i)
 #pragma unroll
                 for (int w = 0; w < kJ / 2; ++w) {
-                    uint32_t word;
-                    if constexpr (kEight) word = two_bf16(tile.v[h][i][w >> 1], tile.v_scale[h][i], w & 1);
-                    else word = tile.v[h][i][w];
-                    wide[h][i][w] = ok ? word : 0;
+                    if constexpr (kEight)
+                        wide[h][i][w] = two_bf16(tile.v[h][i][w >> 1], tile.v_scale[h][kWhole ? 0 : i], w & 1);
+                    else
+                        wide[h][i][w] = tile.v[h][i][w];
                 }
-            }
+        if (ragged) {       // what is not seen may hold anything: 0 * NaN is NaN
+#pragma unroll
+            for (int t = 0; t < 8; ++t)
+#pragma unroll
+                for (int w = 0; w < kJ / 2; ++w)
+                    wide[t >> 2][t & 3][w] = seen >> t & 1 ? wide[t >> 2][t & 3][w] : 0;
+        }
 #pragma unroll
         for (int j = 0; j < kJ; ++j) {
             u32x4 tokens;
@@ -426,7 +504,7 @@ __global__ __launch_bounds__(kWaves * 64) void attend_row_kernel(Attend a) {
         }
     }
 
-    // The waves' parts join in LDS: sums [wave][head][width], then the largest scores and totals.
+    // The waves of a key head join in LDS: sums [wave][head][width], then the largest scores and totals.
     extern __shared__ float shared[];
     float* const tops = shared + kWaves * heads * width;
     float* const totals = tops + kWaves * kHeadTile;
@@ -446,14 +524,13 @@ __global__ __launch_bounds__(kWaves * 64) void attend_row_kernel(Attend a) {
         }
     }
     __syncthreads();
-    for (int at = threadIdx.x * 2; at < heads * width; at += kWaves * 64 * 2) {
+    for (int at = (turn * 64 + lane) * 2; at < heads * width; at += in_turn * 64 * 2) {
         const int head = at / width, d = at - head * width;
         float most = -__builtin_inff();
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) most = __builtin_fmaxf(most, tops[w * kHeadTile + head]);
+        for (int w = wave % beside; w < kWaves; w += beside)
+            most = __builtin_fmaxf(most, tops[w * kHeadTile + head]);
         float x = 0, y = 0, all = 0;
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
+        for (int w = wave % beside; w < kWaves; w += beside) {
             const float mine = tops[w * kHeadTile + head];
             const float share = mine == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((mine - most) * factor);
             const float* const from = shared + (w * heads + head) * width + d;
@@ -462,15 +539,15 @@ __global__ __launch_bounds__(kWaves * 64) void attend_row_kernel(Attend a) {
             all += totals[w * kHeadTile + head] * share;
         }
         if (parts > 1) {
-            const int64_t at_part = (int64_t(sequence) * a.heads + first_head + head) * a.rows.chunks + part;
+            const int64_t at_part = (int64_t(blockIdx.x) * beside + wave % beside) * a.slots + head;
             *reinterpret_cast<float2*>(a.row_parts.sums + at_part * width + d) = float2{x, y};
             if (d == 0) *reinterpret_cast<float2*>(a.row_parts.totals + at_part * 2) = float2{most, all};
         } else {
+            typedef Q Two __attribute__((ext_vector_type(2)));
             const float share = over(all);
-            Q* const to = static_cast<Q*>(a.out) + row * a.out_token_stride +
-                          (first_head + head) * a.out_head_stride + d;
-            to[0] = static_cast<Q>(x * share);
-            to[1] = static_cast<Q>(y * share);
+            *reinterpret_cast<Two*>(static_cast<Q*>(a.out) + row * a.out_token_stride +
+                                    (first_head + head) * a.out_head_stride + d) =
+                Two{static_cast<Q>(x * share), static_cast<Q>(y * share)};
             if (a.lse && d == 0)
                 a.lse[int64_t(row) * a.heads + first_head + head] = most * a.scale + __builtin_logf(all);
         }
@@ -842,62 +919,99 @@ __global__ __launch_bounds__(kTileWaves * 64, kD <= 128 ? 2 : 1) void attend_til
 
 // ----------------------------------------------------------------- parts joined
 
-// The parts of a row's head: a workgroup's threads take values along the row.  The first `alone` workgroups take the
-// sequences of one row, the others the rows of tiles.
+constexpr int kJoinThreads = 256;
+
+// `parts` parts of a row's head, `stride` heads apart, to its out.  A workgroup's threads take four values each, and
+// groups of them parts in turn with a running largest score; the groups join in LDS.  The partial sums come from other
+// dies' caches, about 2 us away: what counts is few steps in a row.
 template <typename Q>
-__global__ __launch_bounds__(256) void join_kernel(Attend a, uint32_t alone) {
-    const bool single = blockIdx.x < alone;
-    const uint32_t job = single ? blockIdx.x : blockIdx.x - alone;
-    const int head = job % a.heads;
-    int sequence = job / a.heads, row = job / a.heads;
-    if (!single) sequence = find_sequence(a.q.n_seqs, row, [&](int s) { return int64_t(a.q.query_starts[s]); });
-    const Rows rows = rows_of(a.q, sequence, a.tokens);
-    if (single) row = rows.first;
-    const int mine = row - rows.first;
-    if (mine < 0 || mine >= rows.count || (rows.count == 1) != single) return;
-    const int width = a.layer.width;
-    const int64_t index = int64_t(row) * a.heads + head;
-    int parts;
-    const float *from, *about;
-    if (single) {
-        parts = parts_of<kTile>(a.rows, sight_of(a, sequence, rows, 0, 0));
-        const int64_t first = (int64_t(sequence) * a.heads + head) * a.rows.chunks;
-        from = a.row_parts.sums + first * width, about = a.row_parts.totals + first * 2;
-    } else {
-        const int pair = mine * a.group + head % a.group;
-        parts = parts_of<kTileTokens>(a.tiles, tile_sight(a, sequence, rows, pair / kTileRows * kTileRows));
-        const int64_t first = index * a.tiles.chunks;
-        from = a.tile_parts.sums + first * width, about = a.tile_parts.totals + first * 2;
-    }
-    if (parts < 2) return;                                  // written by the one workgroup that took it
+__device__ __forceinline__ void join(const Attend& a, const float* from, const float* about, int64_t stride, int parts,
+                                     int row, int head) {
+    const int width = a.layer.width, lanes = width >> 2;
+    const int group = a.quarter_width.divide(threadIdx.x), groups = kJoinThreads / lanes;
+    const int d = (threadIdx.x - group * lanes) * 4;
     const float factor = a.scale * kLog2e;
-    float most = -__builtin_inff();
-    for (int c = 0; c < parts; ++c) most = __builtin_fmaxf(most, about[2 * c]);
-    for (int d = threadIdx.x; d < width; d += 256) {
-        float x = 0, all = 0;
-        for (int c = 0; c < parts; ++c) {
-            const float mine_of = about[2 * c];
-            const float share = mine_of == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((mine_of - most) * factor);
-            x += from[c * width + d] * share;
-            all += about[2 * c + 1] * share;
+    float top = -__builtin_inff(), total = 0;
+    f32x4 x = {0, 0, 0, 0};
+    if (group < groups) {
+        const int64_t first = group * stride;
+        from += first * width + d;
+        about += first * 2;
+#pragma unroll 4
+        for (int c = group; c < parts; c += groups) {
+            const float2 mine = *reinterpret_cast<const float2*>(about);
+            const f32x4 some = *reinterpret_cast<const f32x4*>(from);
+            from += groups * stride * width;
+            about += groups * stride * 2;
+            const float grown = __builtin_fmaxf(top, mine.x);
+            const float against = grown == -__builtin_inff() ? 0.0f : grown;
+            const float keep = __builtin_amdgcn_exp2f((top - against) * factor);
+            const float share = __builtin_amdgcn_exp2f((mine.x - against) * factor);
+            top = grown;
+            total = total * keep + mine.y * share;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) x[k] = x[k] * keep + some[k] * share;
         }
-        static_cast<Q*>(a.out)[row * a.out_token_stride + head * a.out_head_stride + d] = static_cast<Q>(x * over(all));
-        if (a.lse && d == 0) a.lse[index] = most * a.scale + __builtin_logf(all);
     }
+    __shared__ f32x4 sums[kJoinThreads];
+    __shared__ float2 tops[kJoinThreads];
+    sums[threadIdx.x] = x;
+    tops[threadIdx.x] = float2{top, total};
+    __syncthreads();
+    if (group) return;
+    for (int g = 1; g < groups; ++g) {
+        const float2 mine = tops[threadIdx.x + g * lanes];
+        const f32x4 some = sums[threadIdx.x + g * lanes];
+        const float grown = __builtin_fmaxf(top, mine.x);
+        const float against = grown == -__builtin_inff() ? 0.0f : grown;
+        const float keep = __builtin_amdgcn_exp2f((top - against) * factor);
+        const float share = __builtin_amdgcn_exp2f((mine.x - against) * factor);
+        top = grown;
+        total = total * keep + mine.y * share;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[k] = x[k] * keep + some[k] * share;
+    }
+    typedef Q Four __attribute__((ext_vector_type(4)));
+    Four four;
+    const float share = over(total);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) four[k] = static_cast<Q>(x[k] * share);
+    *reinterpret_cast<Four*>(static_cast<Q*>(a.out) + row * a.out_token_stride + head * a.out_head_stride + d) = four;
+    if (a.lse && d == 0) a.lse[int64_t(row) * a.heads + head] = top * a.scale + __builtin_logf(total);
+}
+
+template <typename Q>
+__global__ __launch_bounds__(kJoinThreads) void join_rows_kernel(Attend a) {
+    const int sequence = a.all_heads.divide(blockIdx.x), head = blockIdx.x - sequence * a.heads;
+    const Rows rows = rows_of(a.q, sequence, a.tokens);
+    if (rows.count != 1) return;
+    const int head_groups = a.layer.kv_heads / a.beside * a.head_tiles;
+    const int kv_head = a.group_size.divide(head), of_key = head - kv_head * a.group;
+    const int group_of = kv_head / a.beside * a.head_tiles + of_key / kHeadTile;
+    const int2 info = a.row_info[int64_t(sequence) * head_groups + group_of];
+    if (info.y < 2) return;                                 // written by the one workgroup that took it
+    const int64_t first = (int64_t(info.x + group_of) * a.beside + kv_head % a.beside) * a.slots + of_key % kHeadTile;
+    join<Q>(a, a.row_parts.sums + first * a.layer.width, a.row_parts.totals + first * 2,
+            int64_t(head_groups) * a.beside * a.slots, info.y, rows.first, head);
+}
+
+template <typename Q>
+__global__ __launch_bounds__(kJoinThreads) void join_tiles_kernel(Attend a) {
+    const int row = a.all_heads.divide(blockIdx.x), head = blockIdx.x - row * a.heads;
+    const int sequence = find_sequence(a.q.n_seqs, row, [&](int s) { return int64_t(a.q.query_starts[s]); });
+    const Rows rows = rows_of(a.q, sequence, a.tokens);
+    const int mine = row - rows.first;
+    if (mine < 0 || mine >= rows.count || rows.count == 1) return;
+    const int pair = mine * a.group + (head - a.group_size.divide(head) * a.group);
+    const int parts = parts_of<kTileTokens>(a.tiles, tile_sight(a, sequence, rows, pair / kTileRows * kTileRows));
+    if (parts < 2) return;
+    const int64_t first = (int64_t(row) * a.heads + head) * a.tiles.chunks;
+    join<Q>(a, a.tile_parts.sums + first * a.layer.width, a.tile_parts.totals + first * 2, 1, parts, row, head);
 }
 
 // ----------------------------------------------------------------- launches
 
-// A row's tokens in parts, so that `jobs` rows fill the chip.
-Split split_rows(int64_t jobs, int64_t longest) {
-    constexpr int64_t step = kTile * kWaves, least = 4 * step, wanted = 2048;
-    longest = std::max<int64_t>(longest, 1);
-    int64_t chunk = std::max(least, longest * jobs / wanted);
-    chunk = std::min<int64_t>((chunk + step - 1) / step * step, 1 << 29);
-    return Split{static_cast<int>(chunk), static_cast<int>((longest + kTile - 1 + chunk - 1) / chunk)};
-}
-
-// The same for tiles of rows: whole where there are tiles for two workgroups a CU.
+// A tile of rows' tokens in parts: whole where there are tiles for two workgroups a CU.
 Split split_tiles(int64_t jobs, int64_t longest) {
     constexpr int64_t least = 8 * kTileTokens, wanted = 1024;
     longest = std::max<int64_t>(longest, 1);
@@ -908,16 +1022,55 @@ Split split_tiles(int64_t jobs, int64_t longest) {
 }
 
 struct Plan {
-    Split rows, tiles;
-    int64_t tile_slots, row_parts, tile_parts;  // parts: of all heads, 0 where rows are whole
+    RowJobs rows;
+    Split tiles;
+    int beside, slots;
+    int64_t row_infos = 0, row_jobs, tile_slots, row_parts, tile_parts;  // parts: of all heads, 0 where rows are whole
 };
 
-Plan plan_of(int64_t tokens, int n_seqs, bool ragged, int heads, int kv_heads, int64_t max_length, int64_t window) {
+// How the rows alone are cut, as measured with 32 query heads, 8 key heads of 128 and blocks of 16 tokens.
+//
+// 8 waves side by side read a token's 8 key heads, which lie side by side, at about the same time: 64 ragged sequences
+// of up to 8k tokens in e4m3 (322 MB) take 76 us with 8 heads beside, 79 with 4 and 104 with one.  Few rows are better
+// off with all the waves on one head: the parts are joined in LDS, and one of 32k tokens takes 24.6 us, not 30.9.
+constexpr int kFewHeads = 16;
+// Jobs that the sequences' tokens are cut into: in e4m3 what the chip holds at once, so that all end together (76 us
+// with 450, 88 with 600); a 16-bit cache's jobs are longer, and twice as many are better (135 us, 152 with 500).
+constexpr int kJobsE4m3 = 450, kJobs16 = 1000;
+// Tiles of a wave up to which a row is not cut, the join being 4 to 6 us, and of a part at least.
+constexpr int kWholeTurns = 5, kLeastTurns = 2;
+// Sequences that a wave goes over, 64 at a time, to cut their tokens evenly; more have parts of one length, by the
+// longest.
+constexpr int kEvenSeqs = 256;
+
+Plan plan_of(int64_t tokens, int n_seqs, bool ragged, int heads, int kv_heads, bool eight, int64_t max_length,
+             int64_t window) {
     const int64_t longest = window > 0 ? std::min(window, max_length) : max_length;
     const int64_t group = heads / kv_heads, head_tiles = (group + kHeadTile - 1) / kHeadTile;
     Plan plan{};
-    plan.rows = split_rows(n_seqs * head_tiles * kv_heads, longest);
-    plan.row_parts = plan.rows.chunks < 2 ? 0 : int64_t(n_seqs) * heads * plan.rows.chunks;
+    plan.beside = 1;
+    if (n_seqs * int64_t(kv_heads) >= kFewHeads)
+        while (plan.beside < kWaves && kv_heads % (2 * plan.beside) == 0) plan.beside *= 2;
+    plan.slots = static_cast<int>(std::min<int64_t>(group, kHeadTile));
+    const int64_t row_jobs = n_seqs * head_tiles * (kv_heads / plan.beside);
+    const int64_t tiles = std::max<int64_t>((longest + kTile - 1) / kTile + 1, 1);
+    const int64_t in_turn = kWaves / plan.beside;
+    const int64_t least = kLeastTurns * in_turn, whole = kWholeTurns * in_turn;
+    const int wanted = eight ? kJobsE4m3 : kJobs16;
+    plan.rows = RowJobs{0, 1 << 24, 1, wanted};
+    plan.row_jobs = row_jobs;
+    if (tiles > whole && n_seqs <= kEvenSeqs) {
+        plan.rows.even = 1;
+        plan.rows.chunk = static_cast<int>(least);
+        plan.row_jobs += wanted;
+        plan.row_parts = plan.row_jobs * plan.beside * plan.slots;
+    } else if (tiles > whole) {
+        plan.rows.chunk = static_cast<int>(std::min<int64_t>(std::max(least, tiles * row_jobs / (2 * wanted)), 1 << 24));
+        plan.rows.chunks = static_cast<int>((tiles + plan.rows.chunk - 1) / plan.rows.chunk);
+        plan.row_jobs *= plan.rows.chunks;
+        if (plan.rows.chunks > 1) plan.row_parts = plan.row_jobs * plan.beside * plan.slots;
+    }
+    if (plan.row_parts) plan.row_infos = row_jobs;
     if (ragged) {
         plan.tile_slots = tokens * group / kTileRows + n_seqs;
         // A tile's rows see from the first's window to the last's own token.
@@ -929,15 +1082,16 @@ Plan plan_of(int64_t tokens, int n_seqs, bool ragged, int heads, int kv_heads, i
 }
 
 size_t bytes_of(const Plan& plan, int width) {
-    return static_cast<size_t>(plan.row_parts + plan.tile_parts) * (width + 2) * sizeof(float);
+    return static_cast<size_t>(plan.row_parts + plan.tile_parts) * (width + 2) * sizeof(float) +
+           static_cast<size_t>(plan.row_infos) * sizeof(int2);
 }
 
 template <typename Q, bool kEight, int kJ>
 void launch_rows_of(const Attend& a, unsigned grid, unsigned lds, hipStream_t stream) {
-    if (a.layer.block_size % 16 == 0)
-        hipLaunchKernelGGL((attend_row_kernel<Q, kEight, kJ, true>), dim3(grid), dim3(kWaves * 64), lds, stream, a);
-    else
-        hipLaunchKernelGGL((attend_row_kernel<Q, kEight, kJ, false>), dim3(grid), dim3(kWaves * 64), lds, stream, a);
+    const auto kernel = a.layer.block_size % 16     ? attend_row_kernel<Q, kEight, kJ, false, false>
+                        : a.layer.width == 16 * kJ ? attend_row_kernel<Q, kEight, kJ, true, true>
+                                                   : attend_row_kernel<Q, kEight, kJ, true, false>;
+    hipLaunchKernelGGL(kernel, dim3(grid), dim3(kWaves * 64), lds, stream, a);
 }
 
 template <typename Q, bool kEight>
@@ -971,16 +1125,19 @@ void launch_attend(const Attend& a, const Plan& plan, hipStream_t stream) {
         else launch_tiles<Q, false>(a, grid, stream);
         check_launched("attend's tiles");
     }
-    const unsigned grid = checked_grid(int64_t(a.q.n_seqs) * a.rows.chunks * a.head_tiles * a.layer.kv_heads);
+    const unsigned grid = checked_grid(plan.row_jobs);
     const unsigned lds = 4u * (kWaves * std::min(kHeadTile, a.group) * a.layer.width + 2 * kWaves * kHeadTile);
     if (eight) launch_rows<Q, true>(a, grid, lds, stream);
     else launch_rows<Q, false>(a, grid, lds, stream);
     check_launched("attend");
-    if (plan.row_parts + plan.tile_parts) {
-        const int64_t alone = plan.row_parts ? int64_t(a.q.n_seqs) * a.heads : 0;
-        const int64_t others = plan.tile_parts ? int64_t(a.tokens) * a.heads : 0;
-        hipLaunchKernelGGL(join_kernel<Q>, dim3(checked_grid(alone + others)), dim3(256), 0, stream, a,
-                           static_cast<uint32_t>(alone));
+    if (plan.row_parts) {
+        hipLaunchKernelGGL(join_rows_kernel<Q>, dim3(checked_grid(int64_t(a.q.n_seqs) * a.heads)), dim3(kJoinThreads), 0,
+                           stream, a);
+        check_launched("attend's join");
+    }
+    if (plan.tile_parts) {
+        hipLaunchKernelGGL(join_tiles_kernel<Q>, dim3(checked_grid(int64_t(a.tokens) * a.heads)), dim3(kJoinThreads), 0,
+                           stream, a);
         check_launched("attend's join");
     }
 }
@@ -989,10 +1146,12 @@ void launch_attend(const Attend& a, const Plan& plan, hipStream_t stream) {
 
 extern "C" {
 
-size_t kvsnap_attend_workspace_bytes(int64_t tokens, int n_seqs, int ragged, int heads, int kv_heads, int width,
+size_t kvsnap_attend_workspace_bytes(const kvsnap_paged_layer* layer, int64_t tokens, int n_seqs, int ragged, int heads,
                                      int64_t max_length, int64_t window) {
-    if (tokens <= 0 || n_seqs <= 0 || heads <= 0 || kv_heads <= 0) return 0;
-    return bytes_of(plan_of(tokens, n_seqs, ragged, heads, kv_heads, max_length, window), width);
+    if (!layer || tokens <= 0 || n_seqs <= 0 || heads <= 0 || layer->kv_heads <= 0) return 0;
+    return bytes_of(plan_of(tokens, n_seqs, ragged, heads, layer->kv_heads, layer->type == KVSNAP_E4M3, max_length,
+                            std::min<int64_t>(window, 1 << 30)),
+                    layer->width);
 }
 
 int kvsnap_attend(const kvsnap_paged_layer* layer, const kvsnap_sequences* sequences, const void* query,
@@ -1029,17 +1188,21 @@ int kvsnap_attend(const kvsnap_paged_layer* layer, const kvsnap_sequences* seque
         a.tokens = static_cast<int>(tokens), a.heads = heads, a.group = heads / layer->kv_heads;
         a.scale = scale;
         a.window = static_cast<int>(std::min<int64_t>(window, 1 << 30));
-        a.head_tiles = (a.group + kHeadTile - 1) / kHeadTile;
-        a.block_size = Divider::of(layer->block_size);
-        a.group_size = Divider::of(a.group);
         const int64_t named = int64_t(sequences->table_width) * layer->block_size;
         const Plan plan = plan_of(tokens, sequences->n_seqs, sequences->query_starts != nullptr, heads,
-                                  layer->kv_heads, std::min(max_length, named), a.window);
+                                  layer->kv_heads, layer->type == KVSNAP_E4M3, std::min(max_length, named), a.window);
+        a.head_tiles = (a.group + kHeadTile - 1) / kHeadTile;
+        a.beside = plan.beside, a.slots = plan.slots;
+        a.block_size = Divider::of(layer->block_size);
+        a.group_size = Divider::of(a.group);
+        a.all_heads = Divider::of(heads);
+        a.quarter_width = Divider::of(layer->width / 4);
         a.rows = plan.rows, a.tiles = plan.tiles;
         float* const room = static_cast<float*>(workspace);
         const int64_t parts = plan.row_parts + plan.tile_parts;
         a.row_parts = Parts{room, room + parts * layer->width};
         a.tile_parts = Parts{room + plan.row_parts * layer->width, a.row_parts.totals + plan.row_parts * 2};
+        if (plan.row_infos) a.row_info = reinterpret_cast<int2*>(room + parts * (layer->width + 2));
         require(workspace_bytes >= bytes_of(plan, layer->width), "attend: the workspace is too small");
         require(parts == 0 || (workspace && reinterpret_cast<uintptr_t>(workspace) % 16 == 0),
                 "attend: the workspace must be 16-byte aligned device memory");

@@ -364,9 +364,8 @@ PyObject* attend(PyObject*, PyObject* const* args, Py_ssize_t count) {
         check_device(layer.device, {&query, &out, s.tables, s.lengths, s.starts});
         at::Tensor lse, scratch;
         if (wants_lse) lse = at::empty({tokens, heads}, query.options().dtype(at::kFloat));
-        const size_t size = library.workspace_bytes(tokens, s.raw.n_seqs, s.starts != nullptr,
-                                                    static_cast<int>(heads), static_cast<int>(kv_heads),
-                                                    static_cast<int>(width), longest, window);
+        const size_t size = library.workspace_bytes(layer.raw, tokens, s.raw.n_seqs, s.starts != nullptr,
+                                                    static_cast<int>(heads), longest, window);
         if (size) scratch = at::empty({static_cast<int64_t>(size)}, query.options().dtype(at::kByte));
         launched(layer.device, [&](uintptr_t stream) {
             return library.attend(layer.raw, &s.raw, query.data_ptr(), query.stride(0), query.stride(1),

@@ -77,7 +77,7 @@ KERNEL_SIGNATURES = {
     "kvsnap_hold_stream": "int <- stream int",
     "kvsnap_rotate": "int <- ptr i64 i64 ptr i64 i64 i64 int int int ptr stream",
     "kvsnap_append": "int <- ptr ptr ptr ptr i64 i64 ptr i64 i64 ptr i64 i64 ptr i64 i64 i64 int int stream",
-    "kvsnap_attend_workspace_bytes": "size <- i64 int int int int int i64 i64",
+    "kvsnap_attend_workspace_bytes": "size <- ptr i64 int int int i64 i64",
     "kvsnap_attend": "int <- ptr ptr ptr i64 i64 ptr i64 i64 ptr i64 int int f32 i64 i64 ptr size stream",
 }
 

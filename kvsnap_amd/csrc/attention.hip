@@ -578,7 +578,7 @@ __device__ __forceinline__ uint32_t not_finite(uint32_t word) {
 //
 // K's rows are 16 bytes longer than the values (an odd number of 16-byte pieces: 16-byte reads down a column of rows
 // meet every bank), V's 32 (four rows' 32-byte pieces side by side, what one transposing read takes).
-template <typename Q, bool kEight, int kD>
+template <typename Q, bool kEight, int kD, bool kWhole>
 __global__ __launch_bounds__(kTileWaves * 64, kD <= 128 ? 2 : 1) void attend_tile_kernel(Attend a) {
     using T = typename Shape<Q, kEight>::T;
     using Vec = typename Matrix<T>::Vec;
@@ -586,7 +586,9 @@ __global__ __launch_bounds__(kTileWaves * 64, kD <= 128 ? 2 : 1) void attend_til
     constexpr int kBytes = kEight ? 1 : 2;
     constexpr int kSteps = kD / 16, kBlocks = kD / 32;
     constexpr int kPieces = kD / 8;                         // of eight values, of a row
-    constexpr int kLoads = kTileTokens * kPieces / (kTileWaves * 64);
+    // Threads side by side along a row, so that a wave's rows lie in one group of 16 tokens.
+    constexpr int kBeside = kPieces <= 8 ? 8 : kPieces <= 16 ? 16 : 32;
+    constexpr int kLoads = kTileTokens * kBeside / (kTileWaves * 64);
     constexpr int kKeyRow = kD * 2 + 16, kValueRow = kD * 2 + 32;
     constexpr int kStage = kTileTokens * (kKeyRow + kValueRow);
     constexpr uint32_t kNowhere = ~0u;
@@ -657,52 +659,96 @@ __global__ __launch_bounds__(kTileWaves * 64, kD <= 128 ? 2 : 1) void attend_til
     const char* const values = static_cast<const char*>(a.layer.value) + kv_head * a.layer.head_stride * kBytes;
     const uint8_t* const scales = kEight ? a.layer.scales + kv_head * a.layer.scale_head_stride : nullptr;
 
-    // Lane i's token of the 64 at `token`: where its rows are, in 16 bytes, and its block's scales.
-    struct Place {
-        uint32_t at;
-        float k_scale, v_scale;
-    };
-    const auto place_of = [&](int token) {
-        const int mine = token + lane;
-        Place place{kNowhere, 0, 0};
+    // Where 64 tokens' rows are: lane i has token i's block, or (kWhole: a block is whole groups of 16 tokens) that of
+    // group i & 3.  The table is read two stages ahead of its use, a stage ahead of the rows, so that no wait for it is
+    // a wait for them.
+    const auto named_block = [&](int token) {
+        const int mine = token + (kWhole ? (lane & 3) * 16 : lane);
         const uint32_t page = a.block_size.divide(mine);
-        if (mine < sight.low || mine >= stop || page >= static_cast<uint32_t>(a.q.table_width)) return place;
-        const int block = table[page];
-        if (static_cast<uint32_t>(block) >= static_cast<uint64_t>(a.layer.blocks)) return place;
-        const int slot = mine - page * a.block_size.d;
-        place.at = static_cast<uint32_t>((block * a.layer.block_stride + slot * a.layer.token_stride) * kBytes >> 4);
-        if constexpr (kEight) {
-            const uint8_t* const scale = scales + block * a.layer.scale_block_stride;
-            place.k_scale = power_of(scale[0]);
-            place.v_scale = power_of(scale[a.layer.scale_side_stride]);
-        }
-        return place;
+        int block = -1;
+        if (mine + (kWhole ? 15 : 0) >= sight.low && mine < stop && page < static_cast<uint32_t>(a.q.table_width))
+            block = table[page];
+        return block;
     };
-    // A thread's pieces of a stage: piece thread + 256 i, in the order of rows.
+    struct Places {
+        uint32_t at;                                        // in 16 bytes; kNowhere: in no block, or out of the part
+        uint32_t k_scale, v_scale;                          // e8m0 bytes
+    };
+    const auto places_of = [&](int block, int token) {
+        Places places{kNowhere, 127, 127};
+        if (static_cast<uint32_t>(block) < static_cast<uint64_t>(a.layer.blocks)) {
+            const int mine = token + (kWhole ? (lane & 3) * 16 : lane);
+            const int slot = mine - a.block_size.divide(mine) * a.block_size.d;
+            places.at = static_cast<uint32_t>((block * a.layer.block_stride + slot * a.layer.token_stride) * kBytes >> 4);
+            if constexpr (kEight) {
+                const uint8_t* const scale = scales + block * a.layer.scale_block_stride;
+                places.k_scale = scale[0];
+                places.v_scale = scale[a.layer.scale_side_stride];
+            }
+        }
+        return places;
+    };
+    // Which of the 64 tokens are there.
+    const auto valid_of = [&](const Places& places, int token) -> uint64_t {
+        uint64_t valid = __ballot(places.at != kNowhere);
+        if constexpr (kWhole) {
+            const uint64_t groups = valid & 15;
+            valid = ((groups & 1) | (groups & 2) << 15 | (groups & 4) << 30 | (groups & 8) << 45) * 0xffff;
+            if (token < sight.low) valid &= ~uint64_t(0) << min(sight.low - token, 63);
+            if (token + kTileTokens > stop) valid &= ~uint64_t(0) >> min(kTileTokens - (stop - token), 63);
+        }
+        return valid;
+    };
+    // A thread's pieces of a stage.
+    const int my_row = thread / kBeside, my_piece = thread - my_row * kBeside;
+    const uint32_t my_offset = static_cast<uint32_t>(my_row & 15) * static_cast<uint32_t>(a.layer.token_stride) * kBytes +
+                               my_piece * 8 * kBytes;
+    const bool has_piece = my_piece * 8 < width;
     uint32_t k_words[kLoads][kEight ? 2 : 4], v_words[kLoads][kEight ? 2 : 4];
-    const auto load = [&](const Place& place) {
+    const auto load = [&](const Places& places, uint64_t valid) {
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
-            const int index = thread + i * kTileWaves * 64;
-            const int token = index / kPieces, piece = index - token * kPieces;
-            const uint32_t at = __shfl(place.at, token);
+            const int first_row = i * (kTileWaves * 64 / kBeside), row_of = first_row + my_row;
+            if constexpr (kWhole) {
+                const uint32_t at = __builtin_amdgcn_readlane(places.at, __builtin_amdgcn_readfirstlane(row_of >> 4));
+                const int64_t base_of = (int64_t(at == kNowhere ? 0 : at) << 4) +
+                                        (first_row & 15) * a.layer.token_stride * kBytes;
+                const char* const k_from = keys + base_of;
+                const char* const v_from = values + base_of;
+                if (valid == ~uint64_t(0) && (kPieces == kBeside || has_piece)) {
+                    load_words<kEight ? 2 : 4>(k_from + my_offset, k_words[i]);
+                    load_words<kEight ? 2 : 4>(v_from + my_offset, v_words[i]);
+                } else {
 #pragma unroll
-            for (int w = 0; w < (kEight ? 2 : 4); ++w) k_words[i][w] = v_words[i][w] = 0;
-            if (at != kNowhere && piece * 8 < width) {
-                const int64_t offset = (int64_t(at) << 4) + piece * 8 * kBytes;
-                load_words<kEight ? 2 : 4>(keys + offset, k_words[i]);
-                load_words<kEight ? 2 : 4>(values + offset, v_words[i]);
+                    for (int w = 0; w < (kEight ? 2 : 4); ++w) k_words[i][w] = v_words[i][w] = 0;
+                    if (has_piece && (valid >> row_of & 1)) {
+                        load_words<kEight ? 2 : 4>(k_from + my_offset, k_words[i]);
+                        load_words<kEight ? 2 : 4>(v_from + my_offset, v_words[i]);
+                    }
+                }
+            } else {
+                const uint32_t at = __shfl(places.at, row_of);
+#pragma unroll
+                for (int w = 0; w < (kEight ? 2 : 4); ++w) k_words[i][w] = v_words[i][w] = 0;
+                if (at != kNowhere && has_piece) {
+                    const int64_t offset = (int64_t(at) << 4) + my_piece * 8 * kBytes;
+                    load_words<kEight ? 2 : 4>(keys + offset, k_words[i]);
+                    load_words<kEight ? 2 : 4>(values + offset, v_words[i]);
+                }
             }
         }
     };
-    const auto store = [&](const Place& place, char* to, bool ragged, uint32_t* odd_tokens) {
+    const auto store = [&](const Places& places, char* to, bool ragged, uint32_t* odd_tokens) {
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
-            const int index = thread + i * kTileWaves * 64;
-            const int token = index / kPieces, piece = index - token * kPieces;
+            const int row_of = i * (kTileWaves * 64 / kBeside) + my_row;
             u32x4 k, v;
             if constexpr (kEight) {
-                const float k_scale = __shfl(place.k_scale, token), v_scale = __shfl(place.v_scale, token);
+                const int from = kWhole ? __builtin_amdgcn_readfirstlane(row_of >> 4) : 0;
+                const float k_scale = power_of(kWhole ? __builtin_amdgcn_readlane(places.k_scale, from)
+                                                      : __shfl(places.k_scale, row_of));
+                const float v_scale = power_of(kWhole ? __builtin_amdgcn_readlane(places.v_scale, from)
+                                                      : __shfl(places.v_scale, row_of));
 #pragma unroll
                 for (int w = 0; w < 4; ++w) {
                     k[w] = two_bf16(k_words[i][w >> 1], k_scale, w & 1);
@@ -722,10 +768,12 @@ __global__ __launch_bounds__(kTileWaves * 64, kD <= 128 ? 2 : 1) void attend_til
                     any |= bad;
                     v[w] &= ~bad;
                 }
-                if (any) atomicOr(&odd_tokens[token >> 5], 1u << (token & 31));
+                if (any) atomicOr(&odd_tokens[row_of >> 5], 1u << (row_of & 31));
             }
-            *reinterpret_cast<u32x4*>(to + token * kKeyRow + piece * 16) = k;
-            *reinterpret_cast<u32x4*>(to + kTileTokens * kKeyRow + token * kValueRow + piece * 16) = v;
+            if (my_piece < kPieces) {
+                *reinterpret_cast<u32x4*>(to + row_of * kKeyRow + my_piece * 16) = k;
+                *reinterpret_cast<u32x4*>(to + kTileTokens * kKeyRow + row_of * kValueRow + my_piece * 16) = v;
+            }
         }
     };
     // Whether some of the workgroup's rows see some of the 64 tokens and not others.
@@ -740,15 +788,16 @@ __global__ __launch_bounds__(kTileWaves * 64, kD <= 128 ? 2 : 1) void attend_til
 #pragma unroll
         for (int i = 0; i < 16; ++i) sum[b][i] = 0;
     float top = -__builtin_inff(), total = 0;
-    const float factor = a.scale * kLog2e;
+    const float factor = a.scale * kLog2e, slack = 8.0f / factor;
 
     if (thread < 6) odd[thread >> 1][thread & 1] = 0;
-    Place place = place_of(base);
-    load(place);
-    Place next = place_of(base + kTileTokens);
+    const int block0 = named_block(base);
+    int block = named_block(base + kTileTokens);            // of the next 64 tokens
+    const Places first = places_of(block0, base);
+    uint64_t valid = valid_of(first, base);                 // of the present 64 tokens
+    load(first, valid);
     __syncthreads();
-    store(place, stage, is_ragged(base), odd[0]);
-    uint64_t valid = __ballot(place.at != kNowhere);
+    store(first, stage, is_ragged(base), odd[0]);
     __syncthreads();
 
     int turn = 0;                                           // of three: whose odd tokens
@@ -757,10 +806,13 @@ __global__ __launch_bounds__(kTileWaves * 64, kD <= 128 ? 2 : 1) void attend_til
         const bool more = token + kTileTokens < stop;
         const int turn_next = turn == 2 ? 0 : turn + 1, turn_after = turn_next == 2 ? 0 : turn_next + 1;
         if (thread < 2) odd[turn_after][thread] = 0;
-        Place after_next{kNowhere, 0, 0};
+        Places next{kNowhere, 127, 127};
+        uint64_t valid_next = 0;
         if (more) {
-            load(next);
-            after_next = place_of(token + 2 * kTileTokens);
+            next = places_of(block, token + kTileTokens);
+            valid_next = valid_of(next, token + kTileTokens);
+            block = named_block(token + 2 * kTileTokens);
+            load(next, valid_next);
         }
 
         const bool apart = idle || token > high_position || (a.window > 0 && token + kTileTokens <= low_position - a.window + 1);
@@ -796,7 +848,9 @@ __global__ __launch_bounds__(kTileWaves * 64, kD <= 128 ? 2 : 1) void attend_til
 #pragma unroll
                 for (int i = 0; i < 16; ++i) most = __builtin_fmaxf(most, score[h][i]);
             most = max_across_halves(most);
-            if (__ballot(most > top)) {
+            // Weights are relative to a score at most 2^8 below the largest: they keep their relative precision, and the
+            // sums are scaled again in few tiles.
+            if (__ballot(most > top + slack)) {
                 const float grown = __builtin_fmaxf(top, most);
                 const float shrink = top == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((top - grown) * factor);
                 total *= shrink;
@@ -876,8 +930,7 @@ __global__ __launch_bounds__(kTileWaves * 64, kD <= 128 ? 2 : 1) void attend_til
 
         if (more) {
             store(next, stage + kStage - now, is_ragged(token + kTileTokens), odd[turn_next]);
-            valid = __ballot(next.at != kNowhere);
-            next = after_next;
+            valid = valid_next;
         }
         __syncthreads();
         now = kStage - now;
@@ -1101,14 +1154,20 @@ void launch_rows(const Attend& a, unsigned grid, unsigned lds, hipStream_t strea
     else launch_rows_of<Q, kEight, 16>(a, grid, lds, stream);
 }
 
+template <typename Q, bool kEight, bool kWhole>
+void launch_tiles_of(const Attend& a, unsigned grid, hipStream_t stream) {
+    const auto kernel = a.layer.width <= 64    ? attend_tile_kernel<Q, kEight, 64, kWhole>
+                        : a.layer.width <= 96  ? attend_tile_kernel<Q, kEight, 96, kWhole>
+                        : a.layer.width <= 128 ? attend_tile_kernel<Q, kEight, 128, kWhole>
+                        : a.layer.width <= 192 ? attend_tile_kernel<Q, kEight, 192, kWhole>
+                                               : attend_tile_kernel<Q, kEight, 256, kWhole>;
+    hipLaunchKernelGGL(kernel, dim3(grid), dim3(kTileWaves * 64), 0, stream, a);
+}
+
 template <typename Q, bool kEight>
 void launch_tiles(const Attend& a, unsigned grid, hipStream_t stream) {
-    const auto kernel = a.layer.width <= 64    ? attend_tile_kernel<Q, kEight, 64>
-                        : a.layer.width <= 96  ? attend_tile_kernel<Q, kEight, 96>
-                        : a.layer.width <= 128 ? attend_tile_kernel<Q, kEight, 128>
-                        : a.layer.width <= 192 ? attend_tile_kernel<Q, kEight, 192>
-                                               : attend_tile_kernel<Q, kEight, 256>;
-    hipLaunchKernelGGL(kernel, dim3(grid), dim3(kTileWaves * 64), 0, stream, a);
+    if (a.layer.block_size % 16) launch_tiles_of<Q, kEight, false>(a, grid, stream);
+    else launch_tiles_of<Q, kEight, true>(a, grid, stream);
 }
 
 unsigned checked_grid(int64_t groups) {

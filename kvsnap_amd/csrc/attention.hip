@@ -13,6 +13,7 @@
 #include "paged.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace {
 
@@ -154,6 +155,8 @@ struct Attend {
     int beside;                // key heads that a workgroup's waves take side by side
     int slots;                 // heads of a tile, at most
     Divider block_size, group_size, all_heads, quarter_width;
+    uint32_t block_pieces, token_pieces;      // strides in 16 bytes
+    uint32_t stage_pages, stage_slots;        // pages and slots that 64 tokens go on by
 };
 
 constexpr int kTile = 32;         // tokens a wave takes at a time
@@ -659,33 +662,35 @@ __global__ __launch_bounds__(kTileWaves * 64, kD <= 128 ? 2 : 1) void attend_til
     const char* const values = static_cast<const char*>(a.layer.value) + kv_head * a.layer.head_stride * kBytes;
     const uint8_t* const scales = kEight ? a.layer.scales + kv_head * a.layer.scale_head_stride : nullptr;
 
-    // Where 64 tokens' rows are: lane i has token i's block, or (kWhole: a block is whole groups of 16 tokens) that of
-    // group i & 3.  The table is read two stages ahead of its use, a stage ahead of the rows, so that no wait for it is
-    // a wait for them.
-    const auto named_block = [&](int token) {
-        const int mine = token + (kWhole ? (lane & 3) * 16 : lane);
-        const uint32_t page = a.block_size.divide(mine);
-        int block = -1;
-        if (mine + (kWhole ? 15 : 0) >= sight.low && mine < stop && page < static_cast<uint32_t>(a.q.table_width))
-            block = table[page];
-        return block;
-    };
+    // Where 64 tokens' rows are: lane i has token i's, or (kWhole: a block is whole groups of 16 tokens) those of group
+    // i & 3.  The table is read two stages ahead of its use, a stage ahead of the rows, so that no wait for it is a wait
+    // for them; pages and slots go on from stage to stage.
     struct Places {
         uint32_t at;                                        // in 16 bytes; kNowhere: in no block, or out of the part
         uint32_t k_scale, v_scale;                          // e8m0 bytes
     };
-    const auto places_of = [&](int block, int token) {
+    const int lane_token = kWhole ? (lane & 3) * 16 : lane;
+    uint32_t page = a.block_size.divide(base + lane_token), slot = base + lane_token - page * a.block_size.d;
+    const auto named_block = [&](int token) {               // the table's entry for `page`; -1 where there is none
+        int block = -1;
+        if (token + lane_token + (kWhole ? 15 : 0) >= sight.low && token + lane_token < stop &&
+            page < static_cast<uint32_t>(a.q.table_width))
+            block = table[page];
+        return block;
+    };
+    const auto places_of = [&](int block) {
         Places places{kNowhere, 127, 127};
-        if (static_cast<uint32_t>(block) < static_cast<uint64_t>(a.layer.blocks)) {
-            const int mine = token + (kWhole ? (lane & 3) * 16 : lane);
-            const int slot = mine - a.block_size.divide(mine) * a.block_size.d;
-            places.at = static_cast<uint32_t>((block * a.layer.block_stride + slot * a.layer.token_stride) * kBytes >> 4);
-            if constexpr (kEight) {
+        const bool named = static_cast<uint32_t>(block) < static_cast<uint32_t>(a.layer.blocks);
+        if (named) places.at = static_cast<uint32_t>(block) * a.block_pieces + slot * a.token_pieces;
+        if constexpr (kEight)
+            if (named) {
                 const uint8_t* const scale = scales + block * a.layer.scale_block_stride;
                 places.k_scale = scale[0];
                 places.v_scale = scale[a.layer.scale_side_stride];
             }
-        }
+        page += a.stage_pages;
+        slot += a.stage_slots;
+        if (slot >= a.block_size.d) slot -= a.block_size.d, ++page;
         return places;
     };
     // Which of the 64 tokens are there.
@@ -693,6 +698,7 @@ __global__ __launch_bounds__(kTileWaves * 64, kD <= 128 ? 2 : 1) void attend_til
         uint64_t valid = __ballot(places.at != kNowhere);
         if constexpr (kWhole) {
             const uint64_t groups = valid & 15;
+            if (groups == 15 && token >= sight.low && token + kTileTokens <= stop) return ~uint64_t(0);
             valid = ((groups & 1) | (groups & 2) << 15 | (groups & 4) << 30 | (groups & 8) << 45) * 0xffff;
             if (token < sight.low) valid &= ~uint64_t(0) << min(sight.low - token, 63);
             if (token + kTileTokens > stop) valid &= ~uint64_t(0) >> min(kTileTokens - (stop - token), 63);
@@ -701,40 +707,36 @@ __global__ __launch_bounds__(kTileWaves * 64, kD <= 128 ? 2 : 1) void attend_til
     };
     // A thread's pieces of a stage.
     const int my_row = thread / kBeside, my_piece = thread - my_row * kBeside;
-    const uint32_t my_offset = static_cast<uint32_t>(my_row & 15) * static_cast<uint32_t>(a.layer.token_stride) * kBytes +
-                               my_piece * 8 * kBytes;
+    const uint32_t my_offset = (my_row & 15) * a.token_pieces * 16 + my_piece * 8 * kBytes;
     const bool has_piece = my_piece * 8 < width;
-    uint32_t k_words[kLoads][kEight ? 2 : 4], v_words[kLoads][kEight ? 2 : 4];
+    uint32_t k_words[kLoads][kEight ? 2 : 4] = {}, v_words[kLoads][kEight ? 2 : 4] = {};
     const auto load = [&](const Places& places, uint64_t valid) {
+        if (kWhole && valid == ~uint64_t(0)) {
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                // The wave's group of 16 tokens, and where in it the pass begins.
+                const int first_row = i * (kTileWaves * 64 / kBeside);
+                const int group = (first_row + wave * (64 / kBeside)) >> 4;
+                const int64_t at = (int64_t(__builtin_amdgcn_readlane(places.at, group)) << 4) +
+                                   (first_row & 15) * int64_t(a.token_pieces) * 16;
+                if (kPieces == kBeside || has_piece) {
+                    load_words<kEight ? 2 : 4>(keys + at + my_offset, k_words[i]);
+                    load_words<kEight ? 2 : 4>(values + at + my_offset, v_words[i]);
+                }
+            }
+            return;
+        }
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
-            const int first_row = i * (kTileWaves * 64 / kBeside), row_of = first_row + my_row;
-            if constexpr (kWhole) {
-                const uint32_t at = __builtin_amdgcn_readlane(places.at, __builtin_amdgcn_readfirstlane(row_of >> 4));
-                const int64_t base_of = (int64_t(at == kNowhere ? 0 : at) << 4) +
-                                        (first_row & 15) * a.layer.token_stride * kBytes;
-                const char* const k_from = keys + base_of;
-                const char* const v_from = values + base_of;
-                if (valid == ~uint64_t(0) && (kPieces == kBeside || has_piece)) {
-                    load_words<kEight ? 2 : 4>(k_from + my_offset, k_words[i]);
-                    load_words<kEight ? 2 : 4>(v_from + my_offset, v_words[i]);
-                } else {
+            const int row_of = i * (kTileWaves * 64 / kBeside) + my_row;
+            const uint32_t at = __shfl(places.at, kWhole ? row_of >> 4 : row_of);
 #pragma unroll
-                    for (int w = 0; w < (kEight ? 2 : 4); ++w) k_words[i][w] = v_words[i][w] = 0;
-                    if (has_piece && (valid >> row_of & 1)) {
-                        load_words<kEight ? 2 : 4>(k_from + my_offset, k_words[i]);
-                        load_words<kEight ? 2 : 4>(v_from + my_offset, v_words[i]);
-                    }
-                }
-            } else {
-                const uint32_t at = __shfl(places.at, row_of);
-#pragma unroll
-                for (int w = 0; w < (kEight ? 2 : 4); ++w) k_words[i][w] = v_words[i][w] = 0;
-                if (at != kNowhere && has_piece) {
-                    const int64_t offset = (int64_t(at) << 4) + my_piece * 8 * kBytes;
-                    load_words<kEight ? 2 : 4>(keys + offset, k_words[i]);
-                    load_words<kEight ? 2 : 4>(values + offset, v_words[i]);
-                }
+            for (int w = 0; w < (kEight ? 2 : 4); ++w) k_words[i][w] = v_words[i][w] = 0;
+            if (has_piece && (valid >> row_of & 1)) {
+                const int64_t offset = (int64_t(at + (kWhole ? (row_of & 15) * a.token_pieces : 0)) << 4) +
+                                       my_piece * 8 * kBytes;
+                load_words<kEight ? 2 : 4>(keys + offset, k_words[i]);
+                load_words<kEight ? 2 : 4>(values + offset, v_words[i]);
             }
         }
     };
@@ -744,7 +746,7 @@ __global__ __launch_bounds__(kTileWaves * 64, kD <= 128 ? 2 : 1) void attend_til
             const int row_of = i * (kTileWaves * 64 / kBeside) + my_row;
             u32x4 k, v;
             if constexpr (kEight) {
-                const int from = kWhole ? __builtin_amdgcn_readfirstlane(row_of >> 4) : 0;
+                const int from = (i * (kTileWaves * 64 / kBeside) + wave * (64 / kBeside)) >> 4;
                 const float k_scale = power_of(kWhole ? __builtin_amdgcn_readlane(places.k_scale, from)
                                                       : __shfl(places.k_scale, row_of));
                 const float v_scale = power_of(kWhole ? __builtin_amdgcn_readlane(places.v_scale, from)
@@ -791,107 +793,99 @@ __global__ __launch_bounds__(kTileWaves * 64, kD <= 128 ? 2 : 1) void attend_til
     const float factor = a.scale * kLog2e, slack = 8.0f / factor;
 
     if (thread < 6) odd[thread >> 1][thread & 1] = 0;
-    const int block0 = named_block(base);
-    int block = named_block(base + kTileTokens);            // of the next 64 tokens
-    const Places first = places_of(block0, base);
+    int block = named_block(base);
+    const Places first = places_of(block);
     uint64_t valid = valid_of(first, base);                 // of the present 64 tokens
+    block = named_block(base + kTileTokens);                // of the next 64
     load(first, valid);
+    bool ragged = is_ragged(base);
     __syncthreads();
-    store(first, stage, is_ragged(base), odd[0]);
+    store(first, stage, ragged, odd[0]);
     __syncthreads();
 
-    int turn = 0;                                           // of three: whose odd tokens
-    int now = 0;                                            // the buffer of these tokens
-    for (int token = base; token < stop; token += kTileTokens) {
-        const bool more = token + kTileTokens < stop;
-        const int turn_next = turn == 2 ? 0 : turn + 1, turn_after = turn_next == 2 ? 0 : turn_next + 1;
-        if (thread < 2) odd[turn_after][thread] = 0;
-        Places next{kNowhere, 127, 127};
-        uint64_t valid_next = 0;
-        if (more) {
-            next = places_of(block, token + kTileTokens);
-            valid_next = valid_of(next, token + kTileTokens);
-            block = named_block(token + 2 * kTileTokens);
-            load(next, valid_next);
+    // The products of one wave's rows with 64 tokens.  kSome: not all rows see all tokens.
+    const auto attend = [&](auto some, int token, int now, int turn, uint64_t valid) __attribute__((always_inline)) {
+        constexpr bool kSome = decltype(some)::value;
+        f32x16 score[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) score[h][i] = 0;
+            const char* const from = stage + now + (32 * h + column) * kKeyRow + half * 16;
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s) {
+                const Vec k = *reinterpret_cast<const Vec*>(from + s * 32);
+#pragma unroll
+                for (int t = 0; t < kTerms; ++t) score[h] = Matrix<T>::mul32(k, q[s][t], score[h]);
+            }
         }
-
-        const bool apart = idle || token > high_position || (a.window > 0 && token + kTileTokens <= low_position - a.window + 1);
-        if (!apart) {
-            const bool whole = valid == ~uint64_t(0) && token + kTileTokens - 1 <= low_position &&
-                               (a.window <= 0 || token > high_position - a.window);
-            f32x16 score[2];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) score[h][i] = 0;
-                const char* const from = stage + now + (32 * h + column) * kKeyRow + half * 16;
-#pragma unroll
-                for (int s = 0; s < kSteps; ++s) {
-                    const Vec k = *reinterpret_cast<const Vec*>(from + s * 32);
-#pragma unroll
-                    for (int t = 0; t < kTerms; ++t) score[h] = Matrix<T>::mul32(k, q[s][t], score[h]);
-                }
-            }
-            if (!whole) {
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const int at = 32 * h + 8 * (i >> 2) + 4 * half + (i & 3);
-                        const bool sees = token + at <= position && token + at > after && (valid >> at & 1);
-                        score[h][i] = sees ? score[h][i] : -__builtin_inff();
-                    }
-            }
-            float most = -__builtin_inff();
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) most = __builtin_fmaxf(most, score[h][i]);
-            most = max_across_halves(most);
-            // Weights are relative to a score at most 2^8 below the largest: they keep their relative precision, and the
-            // sums are scaled again in few tiles.
-            if (__ballot(most > top + slack)) {
-                const float grown = __builtin_fmaxf(top, most);
-                const float shrink = top == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((top - grown) * factor);
-                total *= shrink;
-#pragma unroll
-                for (int b = 0; b < kBlocks; ++b)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) sum[b][i] *= shrink;
-                top = grown;
-            }
-            const float against = top == -__builtin_inff() ? 0.0f : top * factor;
-            Vec p[4][kTerms];
+        const bool whole = !kSome || (valid == ~uint64_t(0) && token + kTileTokens - 1 <= low_position &&
+                                      (a.window <= 0 || token > high_position - a.window));
+        if (!whole) {
+            int quad = 4 * half;                        // opaque: what follows from it is not kept for every stage
+            asm volatile("" : "+v"(quad));
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    score[h][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(score[h][i], factor, -against));
-                    total += score[h][i];
-                    const int t = 2 * h + (i >> 3);
-                    if constexpr (kTerms == 2) two_terms(score[h][i], p[t][0], p[t][1], i & 7);
-                    else p[t][0][i & 7] = static_cast<T>(score[h][i]);
+                    const int at = 32 * h + 8 * (i >> 2) + quad + (i & 3);
+                    const bool sees = token + at <= position && token + at > after && (valid >> at & 1);
+                    score[h][i] = sees ? score[h][i] : -__builtin_inff();
                 }
-            // V^T's operand: the four tokens that S^T left side by side, for 16 values by 16 lanes, in one
-            // transposing read.
-            const char* const from = stage + now + kTileTokens * kKeyRow + (4 * half + ((lane & 15) >> 2)) * kValueRow +
-                                     ((lane >> 4 & 1) * 16 + (lane & 3) * 4) * 2;
+        }
+        float most = -__builtin_inff();
 #pragma unroll
-            for (int t = 0; t < 4; ++t)
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int b = 0; b < kBlocks; ++b) {
-                    u32x4 words;
+            for (int i = 0; i < 16; ++i) most = __builtin_fmaxf(most, score[h][i]);
+        most = max_across_halves(most);
+        // Weights are relative to a score at most 2^8 below the largest: they keep their relative precision, and the
+        // sums are scaled again in few tiles.
+        if (__ballot(most > top + slack)) {
+            const float grown = __builtin_fmaxf(top, most);
+            const float shrink = top == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((top - grown) * factor);
+            total *= shrink;
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const auto four = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                            (__attribute__((address_space(3))) short4_t*)(from + (16 * t + 8 * e) * kValueRow + b * 64));
-                        const u32x2 two = bits<u32x2>(four);
-                        words[2 * e] = two[0], words[2 * e + 1] = two[1];
-                    }
+            for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
-                    for (int term = 0; term < kTerms; ++term)
-                        sum[b] = Matrix<T>::mul32(bits<Vec>(words), p[t][term], sum[b]);
+                for (int i = 0; i < 16; ++i) sum[b][i] *= shrink;
+            top = grown;
+        }
+        const float against = top == -__builtin_inff() ? 0.0f : top * factor;
+        Vec p[4][kTerms];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                score[h][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(score[h][i], factor, -against));
+                total += score[h][i];
+                const int t = 2 * h + (i >> 3);
+                if constexpr (kTerms == 2) two_terms(score[h][i], p[t][0], p[t][1], i & 7);
+                else p[t][0][i & 7] = static_cast<T>(score[h][i]);
+            }
+        // V^T's operand: the four tokens that S^T left side by side, for 16 values by 16 lanes, in one
+        // transposing read.
+        const char* const from = stage + now + kTileTokens * kKeyRow + (4 * half + ((lane & 15) >> 2)) * kValueRow +
+                                 ((lane >> 4 & 1) * 16 + (lane & 3) * 4) * 2;
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int b = 0; b < kBlocks; ++b) {
+                u32x4 words;
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const auto four = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                        (__attribute__((address_space(3))) short4_t*)(from + (16 * t + 8 * e) * kValueRow + b * 64));
+                    const u32x2 two = bits<u32x2>(four);
+                    words[2 * e] = two[0], words[2 * e + 1] = two[1];
                 }
+#pragma unroll
+                for (int term = 0; term < kTerms; ++term)
+                    sum[b] = Matrix<T>::mul32(bits<Vec>(words), p[t][term], sum[b]);
+            }
+        if constexpr (kSome) {
+            int quad = 4 * half;
+            asm volatile("" : "+v"(quad));
             const uint64_t odd_tokens = uint64_t(odd[turn][1]) << 32 | odd[turn][0];
             if (odd_tokens) {
                 for (uint64_t left = odd_tokens; left; left &= left - 1) {
@@ -901,7 +895,7 @@ __global__ __launch_bounds__(kTileWaves * 64, kD <= 128 ? 2 : 1) void attend_til
                     for (int h = 0; h < 2; ++h)
 #pragma unroll
                         for (int i = 0; i < 16; ++i)
-                            weight = 32 * h + 8 * (i >> 2) + 4 * half + (i & 3) == at ? score[h][i] : weight;
+                            weight = 32 * h + 8 * (i >> 2) + quad + (i & 3) == at ? score[h][i] : weight;
                     weight = sum_across_halves(weight);
                     const int seen = token + at;
                     const uint32_t page = a.block_size.divide(seen);
@@ -916,7 +910,7 @@ __global__ __launch_bounds__(kTileWaves * 64, kD <= 128 ? 2 : 1) void attend_til
                     for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
-                            const int d = 32 * b + 8 * (i >> 2) + 4 * half + (i & 3);
+                            const int d = 32 * b + 8 * (i >> 2) + quad + (i & 3);
                             if (d >= width || !sees) continue;
                             float x;
                             if constexpr (kEight)
@@ -927,14 +921,41 @@ __global__ __launch_bounds__(kTileWaves * 64, kD <= 128 ? 2 : 1) void attend_til
                 }
             }
         }
+    };
 
+    int turn = 0;                                           // of three: whose odd tokens
+    int now = 0;                                            // the buffer of these tokens
+    int token = base;
+    const auto one_stage = [&](auto some) __attribute__((always_inline)) {
+        constexpr bool kSome = decltype(some)::value;
+        const bool more = token + kTileTokens < stop;
+        Places next{kNowhere, 127, 127};
+        uint64_t valid_next = 0;
         if (more) {
-            store(next, stage + kStage - now, is_ragged(token + kTileTokens), odd[turn_next]);
+            next = places_of(block);
+            valid_next = valid_of(next, token + kTileTokens);
+            block = named_block(token + 2 * kTileTokens);
+            load(next, valid_next);
+        }
+        const int turn_next = turn == 2 ? 0 : turn + 1;
+        if (thread < 2) odd[turn_next == 2 ? 0 : turn_next + 1][thread] = 0;
+        if (!kSome || (!idle && token <= high_position &&
+                       (a.window <= 0 || token + kTileTokens > low_position - a.window + 1)))
+            attend(some, token, now, turn, valid);
+        if (more) {
+            ragged = is_ragged(token + kTileTokens);
+            store(next, stage + kStage - now, ragged, odd[turn_next]);
             valid = valid_next;
         }
         __syncthreads();
         now = kStage - now;
         turn = turn_next;
+        token += kTileTokens;
+    };
+    // In most stages every row sees every token: a loop of their own.
+    while (token < stop) {
+        while (!ragged && valid == ~uint64_t(0) && token < stop) one_stage(std::false_type{});
+        if (token < stop) one_stage(std::true_type{});
     }
 
     total = sum_across_halves(total);
@@ -1255,6 +1276,10 @@ int kvsnap_attend(const kvsnap_paged_layer* layer, const kvsnap_sequences* seque
         a.block_size = Divider::of(layer->block_size);
         a.group_size = Divider::of(a.group);
         a.all_heads = Divider::of(heads);
+        const int64_t element = layer->type == KVSNAP_E4M3 ? 1 : 2;
+        a.block_pieces = static_cast<uint32_t>(layer->block_stride * element / 16);
+        a.token_pieces = static_cast<uint32_t>(layer->token_stride * element / 16);
+        a.stage_pages = kTileTokens / layer->block_size, a.stage_slots = kTileTokens % layer->block_size;
         a.quarter_width = Divider::of(layer->width / 4);
         a.rows = plan.rows, a.tiles = plan.tiles;
         float* const room = static_cast<float*>(workspace);

@@ -121,17 +121,16 @@ __device__ __forceinline__ void turn(const kvsnap_rotation& r, int unit, int64_t
     for (int i = 0; i < kUnit; ++i) v[i] = turned[i];
 }
 
-// One unit of a head from `in` to `out`, turned.
+// One unit of a head, as it comes and as it goes.
 template <typename T>
-__device__ __forceinline__ void turn_unit(const kvsnap_rotation& r, const T* in, T* out, int unit, int64_t token,
-                                          int64_t counted) {
-    const int first = first_run(r, unit), second = second_run(r, unit);
-    float v[kUnit];
-    load8(in + first, v);
-    load8(in + second, v + 8);
-    turn(r, unit, token, counted, v);
-    store8(out + first, v);
-    store8(out + second, v + 8);
+__device__ __forceinline__ void load_unit(const kvsnap_rotation& r, const T* in, int unit, float* v) {
+    load8(in + first_run(r, unit), v);
+    load8(in + second_run(r, unit), v + 8);
+}
+template <typename T>
+__device__ __forceinline__ void store_unit(const kvsnap_rotation& r, T* out, int unit, const float* v) {
+    store8(out + first_run(r, unit), v);
+    store8(out + second_run(r, unit), v + 8);
 }
 
 template <typename T>
@@ -151,7 +150,10 @@ __global__ __launch_bounds__(kLanes) void rotate_kernel(Strided<const T> x, Stri
     if (item >= items) return;
     const uint32_t token = per_token.divide(item), rest = item - token * per_token.d;
     const uint32_t head = units.divide(rest), unit = rest - head * units.d;
-    turn_unit(r, x.row(token, head), out.row(token, head), unit, token, token);
+    float v[kUnit];
+    load_unit(r, x.row(token, head), unit, v);
+    turn(r, unit, token, token, v);
+    store_unit(r, out.row(token, head), unit, v);
 }
 
 // ----------------------------------------------------------------- append
@@ -186,10 +188,13 @@ __device__ __forceinline__ void append_query(const Step<T>& step, const kvsnap_s
     const uint32_t item = min(blockIdx.x * kLanes + threadIdx.x, step.query_items - 1);
     const uint32_t token = step.query_per_token.divide(item), rest = item - token * step.query_per_token.d;
     const uint32_t head = step.units.divide(rest), unit = rest - head * step.units.d;
+    float v[kUnit];
+    load_unit(r, step.query.row(token, head), unit, v);     // under way while the row's position is looked for
     int sequence;
     const int at = locate(q, token, step.tokens, sequence);
     if (at < 0 || blockIdx.x * kLanes + threadIdx.x >= step.query_items) return;
-    turn_unit(r, step.query.row(token, head), step.query_out.row(token, head), unit, token, at);
+    turn(r, unit, token, at, v);
+    store_unit(r, step.query_out.row(token, head), unit, v);
 }
 
 // A 16-bit cache: each unit of a key or value to its slot.
@@ -203,22 +208,29 @@ __global__ __launch_bounds__(kLanes) void append_kernel(Step<T> step, kvsnap_pag
     const uint32_t side_head = step.units.divide(rest), unit = rest - side_head * step.units.d;
     const bool is_value = side_head >= static_cast<uint32_t>(layer.kv_heads);
     const uint32_t head = is_value ? side_head - layer.kv_heads : side_head;
+    float v[kUnit] = {};
+    u32x4 copied[2] = {};
+    if (is_value) {
+        const u32x4* const from = reinterpret_cast<const u32x4*>(step.value.row(token, head) + unit * kUnit);
+        copied[0] = from[0], copied[1] = from[1];
+    } else {
+        load_unit(r, step.key.row(token, head), unit, v);
+    }
     int sequence;
     const int at = locate(q, token, step.tokens, sequence);
     if (at < 0 || index >= step.items) return;
     const uint32_t page = step.block_size.divide(at), slot = at - page * step.block_size.d;
     if (page >= static_cast<uint32_t>(q.table_width)) return;
     const int64_t block = q.block_tables[sequence * q.table_stride + page];
+    if (!is_value) turn(r, unit, token, at, v);
     if (block < 0 || block >= layer.blocks) return;
     T* const cache = static_cast<T*>(is_value ? layer.value : layer.key) + block * layer.block_stride +
                      slot * layer.token_stride + head * layer.head_stride;
     if (is_value) {
-        const T* const from = step.value.row(token, head) + unit * kUnit;
-        const u32x4 x = reinterpret_cast<const u32x4*>(from)[0], y = reinterpret_cast<const u32x4*>(from)[1];
-        reinterpret_cast<u32x4*>(cache + unit * kUnit)[0] = x;
-        reinterpret_cast<u32x4*>(cache + unit * kUnit)[1] = y;
+        reinterpret_cast<u32x4*>(cache + unit * kUnit)[0] = copied[0];
+        reinterpret_cast<u32x4*>(cache + unit * kUnit)[1] = copied[1];
     } else {
-        turn_unit(r, step.key.row(token, head), cache, unit, token, at);
+        store_unit(r, cache, unit, v);
     }
 }
 
@@ -231,9 +243,10 @@ __device__ __forceinline__ int scale_for(float top) {
 }
 
 // An e4m3 cache: a wave takes one head's keys or values in one block, so that the block's scale is one wave's to
-// decide.  It reads the block's new rows twice, for their largest value and to write them (the second time from a
-// cache), 64 / (width / 16) rows at a time.
-template <typename T>
+// decide, 64 / (width / 16) rows at a time.  Blocks of up to kKeep such passes (16 tokens of 128 are two) stay in
+// registers between looking for their largest value and being written; longer ones are read again.  Loads that do not
+// follow from one another are under way together: the table's entry, the rows, their angles.
+template <typename T, int kKeep>
 __global__ __launch_bounds__(kLanes) void append_e4m3_kernel(Step<T> step, kvsnap_paged_layer layer,
                                                              kvsnap_sequences q, kvsnap_rotation r) {
     if (blockIdx.x < step.query_groups) return append_query(step, q, r);
@@ -261,67 +274,94 @@ __global__ __launch_bounds__(kLanes) void append_e4m3_kernel(Step<T> step, kvsna
     const int begin = max(first, page * size), end = min(length, (page + 1) * size);
     if (begin >= end) return;
     const int64_t block = q.block_tables[sequence * q.table_stride + page];
-    if (block < 0 || block >= layer.blocks) return;
 
     const int lane = threadIdx.x & 63;
     const int units = step.units.d, per_pass = 64 / units;
     const int row = step.units.divide(lane), unit = lane - row * units;
     const int run0 = is_value ? unit * kUnit : first_run(r, unit);
     const int run1 = is_value ? unit * kUnit + 8 : second_run(r, unit);
+    const int low = row < per_pass ? begin + row : end;     // lanes past the last whole row take none
     const auto load = [&](int at, float* v) {
         const int64_t token = rows.first + at - first;
         const T* const from = is_value ? step.value.row(token, head) : step.key.row(token, head);
         load8(from + run0, v);
         load8(from + run1, v + 8);
-        if (!is_value) turn(r, unit, token, at, v);
+    };
+    const auto turned = [&](int at, float* v) {
+        if (!is_value) turn(r, unit, rows.first + at - first, at, v);
     };
     float top = 0;
-    for (int at = begin + row; at < end && row < per_pass; at += per_pass) {
-        float v[kUnit];
-        load(at, v);
+    const auto look = [&](const float* v) {
 #pragma unroll
         for (int i = 0; i < kUnit; ++i) {
             const float size_of = __builtin_fabsf(v[i]);
             top = size_of < __builtin_inff() ? __builtin_fmaxf(top, size_of) : top;
         }
-    }
+    };
+    float kept[kKeep > 0 ? kKeep : 1][kUnit];
+    if constexpr (kKeep > 0) {
 #pragma unroll
-    for (int step_of = 1; step_of < 64; step_of <<= 1) top = __builtin_fmaxf(top, __shfl_xor(top, step_of));
-    int scale = scale_for(top);
+        for (int k = 0; k < kKeep; ++k)
+            if (low + k * per_pass < end) load(low + k * per_pass, kept[k]);
+#pragma unroll
+        for (int k = 0; k < kKeep; ++k)
+            if (low + k * per_pass < end) {
+                turned(low + k * per_pass, kept[k]);
+                look(kept[k]);
+            }
+    } else {
+        for (int at = low; at < end; at += per_pass) {
+            float v[kUnit];
+            load(at, v);
+            turned(at, v);
+            look(v);
+        }
+    }
+    if (block < 0 || block >= layer.blocks) return;
     uint8_t* const held = layer.scales + block * layer.scale_block_stride + head * layer.scale_head_stride +
                           (is_value ? layer.scale_side_stride : 0);
     uint8_t* const cache = static_cast<uint8_t*>(is_value ? layer.value : layer.key) + block * layer.block_stride +
                            head * layer.head_stride;
     const int filled = begin - page * size;
-    if (filled > 0) {
-        const int before = *held;
-        scale = max(scale, before);
-        if (scale > before) {
-            // The slots before the new ones, rounded again: a power of two only costs the bits that fall under
-            // e4m3's least value.
-            for (int slot = row; slot < filled && row < per_pass; slot += per_pass) {
-                u32x4* const words = reinterpret_cast<u32x4*>(cache + slot * layer.token_stride + unit * kUnit);
-                u32x4 old = *words;
+    const int before = filled > 0 ? *held : 0;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float v[4];
-                    unpack_e4m3(old[i], v);
+    for (int step_of = 1; step_of < 64; step_of <<= 1) top = __builtin_fmaxf(top, __shfl_xor(top, step_of));
+    const int scale = max(scale_for(top), before);
+    if (filled > 0 && scale > before) {
+        // The slots before the new ones, rounded again: a power of two only costs the bits that fall under e4m3's least
+        // value.
+        for (int slot = row; slot < filled && row < per_pass; slot += per_pass) {
+            u32x4* const words = reinterpret_cast<u32x4*>(cache + slot * layer.token_stride + unit * kUnit);
+            u32x4 old = *words;
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) v[k] = __builtin_amdgcn_ldexpf(v[k], before - scale);
-                    old[i] = pack_e4m3(v);
-                }
-                *words = old;
+            for (int i = 0; i < 4; ++i) {
+                float v[4];
+                unpack_e4m3(old[i], v);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[k] = __builtin_amdgcn_ldexpf(v[k], before - scale);
+                old[i] = pack_e4m3(v);
             }
+            *words = old;
         }
     }
-    for (int at = begin + row; at < end && row < per_pass; at += per_pass) {
-        float v[kUnit];
-        load(at, v);
+    const auto write = [&](int at, float* v) {
 #pragma unroll
         for (int i = 0; i < kUnit; ++i) v[i] = __builtin_amdgcn_ldexpf(v[i], 127 - scale);
         uint8_t* const to = cache + (at - page * size) * layer.token_stride;
         *reinterpret_cast<u32x2*>(to + run0) = u32x2{pack_e4m3(v), pack_e4m3(v + 4)};
         *reinterpret_cast<u32x2*>(to + run1) = u32x2{pack_e4m3(v + 8), pack_e4m3(v + 12)};
+    };
+    if constexpr (kKeep > 0) {
+#pragma unroll
+        for (int k = 0; k < kKeep; ++k)
+            if (low + k * per_pass < end) write(low + k * per_pass, kept[k]);
+    } else {
+        for (int at = low; at < end; at += per_pass) {
+            float v[kUnit];
+            load(at, v);
+            turned(at, v);
+            write(at, v);
+        }
     }
     if (lane == 0) *held = static_cast<uint8_t>(scale);
 }
@@ -388,8 +428,14 @@ void launch_append(const kvsnap_paged_layer& layer, const kvsnap_sequences& q, c
         const int64_t work = q.query_starts ? tokens / layer.block_size + 2 * int64_t(q.n_seqs) : tokens;
         step.items = counted_items(work, layer.kv_heads, 2);
         step.kv_per_token = Divider::of(2 * layer.kv_heads);
-        hipLaunchKernelGGL(append_e4m3_kernel<T>, dim3(step.query_groups + groups_of(step.items, kLanes / 64)),
-                           dim3(kLanes), 0, stream, step, layer, q, r);
+        // Passes over a block, or over the one row that a sequence adds where there are no query_starts.
+        const int passes = q.query_starts ? (layer.block_size + 64 / units - 1) / (64 / units) : 1;
+        const auto kernel = passes == 1   ? append_e4m3_kernel<T, 1>
+                            : passes == 2 ? append_e4m3_kernel<T, 2>
+                            : passes <= 4 ? append_e4m3_kernel<T, 4>
+                                          : append_e4m3_kernel<T, 0>;
+        hipLaunchKernelGGL(kernel, dim3(step.query_groups + groups_of(step.items, kLanes / 64)), dim3(kLanes), 0,
+                           stream, step, layer, q, r);
     } else {
         step.items = counted_items(tokens, 2 * int64_t(layer.kv_heads), units);
         step.kv_per_token = Divider::of(2 * layer.kv_heads * units);

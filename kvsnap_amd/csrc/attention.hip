@@ -580,7 +580,8 @@ __device__ __forceinline__ uint32_t not_finite(uint32_t word) {
 // the next tokens' loads are under way while the present ones' products run, and one barrier parts the two.
 //
 // K's rows are 16 bytes longer than the values (an odd number of 16-byte pieces: 16-byte reads down a column of rows
-// meet every bank), V's 32 (four rows' 32-byte pieces side by side, what one transposing read takes).
+// meet every bank); V's are 64 or 192 bytes past a multiple of 256, so that the 64 bytes of four rows that half a wave's
+// transposing read takes lie side by side over the banks.  No read waits for a bank.
 template <typename Q, bool kEight, int kD, bool kWhole>
 __global__ __launch_bounds__(kTileWaves * 64, kD <= 128 ? 2 : 1) void attend_tile_kernel(Attend a) {
     using T = typename Shape<Q, kEight>::T;
@@ -592,7 +593,7 @@ __global__ __launch_bounds__(kTileWaves * 64, kD <= 128 ? 2 : 1) void attend_til
     // Threads side by side along a row, so that a wave's rows lie in one group of 16 tokens.
     constexpr int kBeside = kPieces <= 8 ? 8 : kPieces <= 16 ? 16 : 32;
     constexpr int kLoads = kTileTokens * kBeside / (kTileWaves * 64);
-    constexpr int kKeyRow = kD * 2 + 16, kValueRow = kD * 2 + 32;
+        constexpr int kKeyRow = kD * 2 + 16, kValueRow = kD * 2 + (kD == 96 ? 0 : 64);
     constexpr int kStage = kTileTokens * (kKeyRow + kValueRow);
     constexpr uint32_t kNowhere = ~0u;
     __shared__ __attribute__((aligned(16))) char stage[2 * kStage];
@@ -993,16 +994,16 @@ __global__ __launch_bounds__(kTileWaves * 64, kD <= 128 ? 2 : 1) void attend_til
 
 // ----------------------------------------------------------------- parts joined
 
-constexpr int kJoinThreads = 256;
+constexpr int kJoinThreads = 256, kJoinTileThreads = 64;
 
 // `parts` parts of a row's head, `stride` heads apart, to its out.  A workgroup's threads take four values each, and
 // groups of them parts in turn with a running largest score; the groups join in LDS.  The partial sums come from other
 // dies' caches, about 2 us away: what counts is few steps in a row.
-template <typename Q>
+template <typename Q, int kThreads>
 __device__ __forceinline__ void join(const Attend& a, const float* from, const float* about, int64_t stride, int parts,
                                      int row, int head) {
     const int width = a.layer.width, lanes = width >> 2;
-    const int group = a.quarter_width.divide(threadIdx.x), groups = kJoinThreads / lanes;
+    const int group = a.quarter_width.divide(threadIdx.x), groups = kThreads / lanes;
     const int d = (threadIdx.x - group * lanes) * 4;
     const float factor = a.scale * kLog2e;
     float top = -__builtin_inff(), total = 0;
@@ -1027,8 +1028,8 @@ __device__ __forceinline__ void join(const Attend& a, const float* from, const f
             for (int k = 0; k < 4; ++k) x[k] = x[k] * keep + some[k] * share;
         }
     }
-    __shared__ f32x4 sums[kJoinThreads];
-    __shared__ float2 tops[kJoinThreads];
+    __shared__ f32x4 sums[kThreads];
+    __shared__ float2 tops[kThreads];
     sums[threadIdx.x] = x;
     tops[threadIdx.x] = float2{top, total};
     __syncthreads();
@@ -1065,12 +1066,12 @@ __global__ __launch_bounds__(kJoinThreads) void join_rows_kernel(Attend a) {
     const int2 info = a.row_info[int64_t(sequence) * head_groups + group_of];
     if (info.y < 2) return;                                 // written by the one workgroup that took it
     const int64_t first = (int64_t(info.x + group_of) * a.beside + kv_head % a.beside) * a.slots + of_key % kHeadTile;
-    join<Q>(a, a.row_parts.sums + first * a.layer.width, a.row_parts.totals + first * 2,
+    join<Q, kJoinThreads>(a, a.row_parts.sums + first * a.layer.width, a.row_parts.totals + first * 2,
             int64_t(head_groups) * a.beside * a.slots, info.y, rows.first, head);
 }
 
 template <typename Q>
-__global__ __launch_bounds__(kJoinThreads) void join_tiles_kernel(Attend a) {
+__global__ __launch_bounds__(kJoinTileThreads) void join_tiles_kernel(Attend a) {
     const int row = a.all_heads.divide(blockIdx.x), head = blockIdx.x - row * a.heads;
     const int sequence = find_sequence(a.q.n_seqs, row, [&](int s) { return int64_t(a.q.query_starts[s]); });
     const Rows rows = rows_of(a.q, sequence, a.tokens);
@@ -1080,16 +1081,16 @@ __global__ __launch_bounds__(kJoinThreads) void join_tiles_kernel(Attend a) {
     const int parts = parts_of<kTileTokens>(a.tiles, tile_sight(a, sequence, rows, pair / kTileRows * kTileRows));
     if (parts < 2) return;
     const int64_t first = (int64_t(row) * a.heads + head) * a.tiles.chunks;
-    join<Q>(a, a.tile_parts.sums + first * a.layer.width, a.tile_parts.totals + first * 2, 1, parts, row, head);
+    join<Q, kJoinTileThreads>(a, a.tile_parts.sums + first * a.layer.width, a.tile_parts.totals + first * 2, 1, parts, row, head);
 }
 
 // ----------------------------------------------------------------- launches
 
 // A tile of rows' tokens in parts: whole where there are tiles for two workgroups a CU.
 Split split_tiles(int64_t jobs, int64_t longest) {
-    constexpr int64_t least = 8 * kTileTokens, wanted = 1024;
+        constexpr int64_t least = 8 * kTileTokens, wanted = 1536, enough = 512;
     longest = std::max<int64_t>(longest, 1);
-    if (jobs >= wanted / 2) return Split{1 << 29, 1};
+    if (jobs >= enough) return Split{1 << 29, 1};
     int64_t chunk = std::max(least, longest * jobs / wanted);
     chunk = std::min<int64_t>((chunk + kTileTokens - 1) / kTileTokens * kTileTokens, 1 << 29);
     return Split{static_cast<int>(chunk), static_cast<int>((longest + kTileTokens - 1 + chunk - 1) / chunk)};
@@ -1216,7 +1217,7 @@ void launch_attend(const Attend& a, const Plan& plan, hipStream_t stream) {
         check_launched("attend's join");
     }
     if (plan.tile_parts) {
-        hipLaunchKernelGGL(join_tiles_kernel<Q>, dim3(checked_grid(int64_t(a.tokens) * a.heads)), dim3(kJoinThreads), 0,
+        hipLaunchKernelGGL(join_tiles_kernel<Q>, dim3(checked_grid(int64_t(a.tokens) * a.heads)), dim3(kJoinTileThreads), 0,
                            stream, a);
         check_launched("attend's join");
     }

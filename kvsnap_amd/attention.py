@@ -49,12 +49,12 @@ def rotary_table(width, positions, *, base=10000.0, device=None):
 
 
 def block_scales(blocks, layers, heads, *, device=None):
-    """Scales of e4m3 caches of ``layers`` layers: one tensor whose rows are whole 8-byte words, so that a plane can
-    save them with their blocks (``TorchBlockDataPlane(..., scales=...)``), and its ``[blocks, heads, 2]`` view for
-    each layer's :class:`PagedCache`."""
+    """Scales of e4m3 caches of ``layers`` layers: one tensor with a row of whole 16-byte words a block, which a plane
+    saves with the block (``TorchBlockDataPlane(..., scales=...)``), and its ``[blocks, heads, 2]`` view for each
+    layer's :class:`PagedCache`."""
     import torch
     used = layers * heads * 2
-    rows = torch.zeros((blocks, -(-used // 8) * 8), dtype=torch.uint8, device=device).view(torch.float8_e8m0fnu)
+    rows = torch.zeros((blocks, -(-used // 16) * 16), dtype=torch.uint8, device=device).view(torch.float8_e8m0fnu)
     return rows, [rows[:, at:at + 2 * heads].unflatten(1, (heads, 2)) for at in range(0, used, 2 * heads)]
 
 

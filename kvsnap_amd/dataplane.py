@@ -32,7 +32,7 @@ import time
 
 from .native import (HIP_LIBRARY_NAME, NATIVE, HostStaging, check as _check, drain as _drain, kernel_library,
                      resolve_cuda_library)
-from .layout import describe_layer, layout_identity
+from .layout import describe_layer, describe_scales, layout_identity
 from .pool import CopyFailed, CudaPool, HipPool, PinnedAllocation, PinnedCapacityError, drop, hold, settle_readers
 
 logger = logging.getLogger(__name__)
@@ -817,10 +817,14 @@ class TorchBlockDataPlane:
     per layer, whose layer segment of a record is its K span followed by its
     V span.  The actual layout is recorded in ``layers`` (the snapshot
     identity); unsupported views fail closed.
+
+    ``scales`` are the scales of e4m3 caches that :class:`kvsnap_amd.attention.PagedCache` fills: one row of bytes a
+    block for all layers (``kvsnap_amd.attention.block_scales``).  A block's row is saved and restored with its block,
+    behind the layers in its record, and named in the identity.
     """
 
     def __init__(self, caches, block_size, capacity_bytes, *, restore_programs=None, gather_programs=None,
-                 save_mode=None, restore_stream=None, restore_mode=None, device_staging_bytes=None):
+                 save_mode=None, restore_stream=None, restore_mode=None, device_staging_bytes=None, scales=None):
         import torch
         if not caches:
             raise ValueError("empty KV cache registration")
@@ -838,6 +842,11 @@ class TorchBlockDataPlane:
         if device.type != "cuda" or any(tensor.device != device for tensor in self.caches.values()):
             raise ValueError("every KV cache must be on one and the same CUDA device")
         self.layers = [describe_layer(name, tensor, block_size) for name, tensor in self.caches.items()]
+        self.scales = scales
+        if scales is not None:
+            if scales.device != device:
+                raise ValueError("the scales must be on the KV caches' device")
+            self.layers.append(describe_scales(scales))
         self.block_bytes = sum(layer["bytes"] for layer in self.layers)
         self.restore_programs = RESTORE_PROGRAMS if restore_programs is None else restore_programs
         self.gather_programs = GATHER_PROGRAMS if gather_programs is None else gather_programs
@@ -882,6 +891,12 @@ class TorchBlockDataPlane:
         """The registered layout as the snapshot identity string (reference ``vllm.py:236``)."""
         return layout_identity(self.layers)
 
+    def paged_cache(self, name, *, scales=None):
+        """The registered cache ``name`` for the operators that fill and read it (``kvsnap_amd.attention``); an e4m3
+        one with its layer's ``scales``."""
+        from .attention import PagedCache
+        return PagedCache(self.caches[name], self.block_size, scales=scales)
+
     def _num_blocks(self, tensor):
         return tensor.shape[1] if tensor.ndim == 5 else tensor.shape[0]
 
@@ -890,7 +905,10 @@ class TorchBlockDataPlane:
         smallest cache's block count."""
         limit = getattr(self, "_block_limit", None)
         if limit is None:
-            limit = self._block_limit = min(self._num_blocks(t) for t in self.caches.values())
+            limit = min(self._num_blocks(t) for t in self.caches.values())
+            if getattr(self, "scales", None) is not None:
+                limit = min(limit, self.scales.shape[0])
+            self._block_limit = limit
         # C-level passes: a generator over 512 ids took 0.08 ms of a restore's 0.4 ms before its first launch.
         if ids and (not set(map(type, ids)) <= {int} or min(ids) < 0 or max(ids) >= limit):
             raise ValueError("GPU block id out of range")
@@ -935,15 +953,22 @@ class TorchBlockDataPlane:
                         raise ValueError(f"KV layer {layer['name']} is not 8-byte aligned for the copy kernels")
                 spans.extend(parts)
                 offset += layer["bytes"]
+            scales = getattr(self, "scales", None)
+            if scales is not None:
+                if scales.data_ptr() % 8:
+                    raise ValueError("the scales are not 8-byte aligned for the copy kernels")
+                spans.append((offset, scales.data_ptr(), scales.stride(0), self.layers[-1]["bytes"]))
             self._span_table = spans
         return self._span_table
 
     @property
     def min_span_bytes(self):
-        """The shortest span's length: the copy launches' shape hint (short spans share a workgroup).  Found once:
-        every launch asks."""
+        """The caches' shortest span's length: the copy launches' shape hint (short spans share a workgroup).  Found
+        once: every launch asks."""
         if getattr(self, "_min_span", None) is None:
-            self._min_span = min(span[3] for span in self.spans())
+            spans = self.spans()
+            self._min_span = min(span[3] for span in (spans[:-1] if getattr(self, "scales", None) is not None
+                                                      else spans))
         return self._min_span
 
     def _copy_stream_handle(self):
@@ -1263,6 +1288,8 @@ class TorchBlockDataPlane:
     def _find_tail_regions(self, valid):
         regions, offset = [], 0
         for layer in self.layers:
+            if len(layer["shape"]) == 1:        # a block's scales: no token slots
+                continue
             if len(layer["shape"]) == 4:       # [2, N, H, C] K/V split
                 _, n, h, c = layer["shape"]
                 _, sn, sh, _ = layer["stride"]
@@ -1342,8 +1369,8 @@ class TorchBlockDataPlane:
         """Whether every span is its token slots one after another, each whole 8-byte words: a partly filled
         block is then the front of each of its spans."""
         if getattr(self, "_tokens_outermost", None) is None:
-            outermost = True
-            for layer in self.layers:
+            outermost = getattr(self, "scales", None) is None       # a block's scales are no token slots
+            for layer in self.layers if outermost else ():
                 half = len(layer["shape"]) == 4           # [2, N, H, C] K/V split, else [H, N, C]
                 n = layer["shape"][1]
                 heads, step = (layer["shape"][2], layer["stride"][1]) if half else (layer["shape"][0],

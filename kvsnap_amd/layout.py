@@ -84,6 +84,17 @@ def describe_layer(name, tensor, block_size):
     return _block_major(name, tensor, block_size)
 
 
+def describe_scales(scales):
+    """The identity entry of e4m3 caches' scales: ``[blocks, bytes]``, a block's bytes (for all layers) contiguous and
+    whole 8-byte words, or ValueError.  They stand behind the layers in a record and have no token slots."""
+    if scales.ndim != 2 or scales.element_size() != 1 or not scales.shape[1] or scales.shape[1] % 8:
+        _refuse("scales", f"{list(scales.shape)} of {scales.dtype}, expected [blocks, bytes], whole 8-byte words of bytes")
+    if scales.stride(1) != 1 or scales.stride(0) < scales.shape[1] or scales.stride(0) % 8:
+        _refuse("scales", "a block's bytes must be contiguous, and blocks whole 8-byte words apart")
+    return {"name": "block scales", "shape": [scales.shape[1]], "dtype": str(scales.dtype), "stride": [1],
+            "bytes": scales.shape[1]}
+
+
 def layout_identity(layers):
     """The snapshot identity string of registered ``layers`` (the reference's kv_layout, vllm.py:236)."""
     return json.dumps(layers, sort_keys=True, separators=(",", ":"))

@@ -181,9 +181,9 @@ def test_a_cache_that_is_no_paged_cache_is_refused(cache, scales, why):
 
 def test_block_scales_are_whole_words_a_block():
     rows, views = block_scales(5, 3, 3)
-    assert rows.shape == (5, 24) and rows.dtype == torch.float8_e8m0fnu and len(views) == 3
+    assert rows.shape == (5, 32) and rows.dtype == torch.float8_e8m0fnu and len(views) == 3
     for i, view in enumerate(views):
-        assert view.shape == (5, 3, 2) and view.data_ptr() == rows.data_ptr() + 6 * i and view.stride() == (24, 2, 1)
+        assert view.shape == (5, 3, 2) and view.data_ptr() == rows.data_ptr() + 6 * i and view.stride() == (32, 2, 1)
 
 
 def test_rotary_table():
@@ -296,3 +296,72 @@ def test_the_workspace_grows_with_what_is_split_and_is_none_for_short_rows():
     assert size(C.addressof(held), 8192, 1, 1, 32, 8192, 0) <= 32 << 20
     assert 0 < size(C.addressof(held), 1, 1, 0, 32, 32768, 0) <= 32 << 20
     assert size(C.addressof(held), 1, 1, 0, 32, 32768, 100) == 0
+
+
+# ---- a plane with scales
+
+
+class Rows:
+    """A row of bytes a block, as a scales tensor describes itself."""
+
+    dtype, ndim = "torch.float8_e8m0fnu", 2
+
+    def __init__(self, shape=(6, 32), strides=None, address=4096, device=None):
+        from types import SimpleNamespace
+        self.shape, self.strides, self.address = shape, strides or (shape[1], 1), address
+        self.device = device or SimpleNamespace(type="cuda", index=0)
+
+    def stride(self, axis):
+        return self.strides[axis]
+
+    def element_size(self):
+        return 1
+
+    def data_ptr(self):
+        return self.address
+
+
+def plane_with(scales):
+    import sys
+    from types import SimpleNamespace
+    from unittest.mock import MagicMock, patch
+    from kvsnap_amd import dataplane
+
+    class Cache:
+        dtype, ndim, shape, strides = "torch.float8_e4m3fn", 4, (8, 2, 16, 128), (4096, 128, 256, 1)
+        device = scales.device
+
+        def stride(self, axis):
+            return self.strides[axis]
+
+        def element_size(self):
+            return 1
+
+        def data_ptr(self):
+            return 1 << 20
+
+    with patch.dict(sys.modules, {"torch": SimpleNamespace()}), \
+         patch.object(dataplane, "CudaPool", return_value=MagicMock()):
+        return dataplane.TorchBlockDataPlane({"layer.0": Cache()}, 16, 4096, scales=scales)
+
+
+def test_a_planes_record_ends_with_the_blocks_scales():
+    plane = plane_with(Rows())
+    assert plane.block_bytes == 4096 + 32 and plane.spans() == [(0, 1 << 20, 4096, 4096), (4096, 4096, 32, 32)]
+    assert plane.min_span_bytes == 4096 and '"block scales"' in plane.layout_identity
+    # the token slots past the last one are zeroed, the scales are not; and the front of every span is no filled block
+    assert plane._tail_regions(15) == [(15 * 256, 256)] and not plane._token_bytes_divide()
+    plane._validate_ids([0, 5])
+    with pytest.raises(ValueError, match="out of range"):
+        plane._validate_ids([6])
+
+
+@pytest.mark.parametrize("scales,why", [
+    (dict(shape=(6, 12)), "whole 8-byte words"), (dict(shape=(6, 0)), "whole 8-byte words"),
+    (dict(strides=(32, 2)), "contiguous"), (dict(strides=(24, 1)), "contiguous"), (dict(strides=(36, 1)), "contiguous"),
+])
+def test_scales_that_a_plane_cannot_save_are_refused(scales, why):
+    with pytest.raises(ValueError, match=why):
+        plane_with(Rows(**scales))
+    with pytest.raises(ValueError, match="8-byte aligned"):
+        plane_with(Rows(address=4100)).spans()

@@ -817,10 +817,17 @@ def run_rotating(args, hashed=None):
     # 41 GB/s with a 0.17 ms p99 decode stall.  The restore kernel reading pinned memory in place holds CUs
     # through the link's latency and stalled the decode 0.85 ms at p99; staged saves (full-grid gathers)
     # moved only 14 GB/s beside it.
+    attended = args.decode == "attention"
+    scale_rows, scale_views = None, [None] * layers
+    if attended:
+        from kvsnap_amd.attention import block_scales
+        scale_rows, scale_views = block_scales(num_blocks, layers, 8, device="cuda")
+        scale_rows.view(torch.uint8).fill_(127)
     plane = TorchBlockDataPlane(caches, block_size, sum(t // block_size for t in sessions_tokens) * size + (64 << 20),
                                 save_mode=args.save_mode or "direct", restore_programs=args.programs or 4,
                                 restore_mode=args.restore_mode or "dma",
-                                gather_programs=args.gather_programs)
+                                gather_programs=args.gather_programs, scales=scale_rows)
+    size = plane.block_bytes
     plane.warm_up()
     scales_rng = random.Random(4)
     layer_inv = [scales_rng.uniform(0.5, 2.0) for _ in range(layers)]
@@ -852,6 +859,18 @@ def run_rotating(args, hashed=None):
     def decode_step():
         _check(lib, lib.kvsnap_synth_decode(bases.data_ptr(), pitches.data_ptr(), words.data_ptr(), len(spans),
                                             table.data_ptr(), seqs, per_seq, out.data_ptr(), 0, compute.cuda_stream))
+
+    if attended:
+        # the sequences' attention itself: one query token each, 16 heads over the 8 key heads, every layer, in a graph
+        paged = [plane.paged_cache(name, scales=view) for name, view in zip(plane.caches, scale_views)]
+        queries = torch.randn((layers, seqs, 16, 128), device="cuda").to(torch.bfloat16)
+        tables, lengths = table.to(torch.int32), torch.full((seqs,), per_seq * block_size, dtype=torch.int32, device="cuda")
+        outs = torch.empty_like(queries)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            for layer, query, to in zip(paged, queries, outs):
+                layer.attend(query, tables, lengths, out=to)
+        decode_step = graph.replay
 
     def run_steps(count=None, until=None, depth=32):
         pairs = []
@@ -907,7 +926,7 @@ def run_rotating(args, hashed=None):
     for *_, staged, _ in sessions:
         staged.close()
     plane.close()
-    step_bytes = seqs * per_seq * len(spans) * (size // len(spans))
+    step_bytes = seqs * per_seq * size
     return {"metric": "rotating fp8 sessions under decode load, Qwen3-1.7B", "workload": "rotating-fp8",
             "value": round(moved[0] / elapsed / 1e9, 3), "unit": "GB/s (copy, beside decode)",
             "copy_alone_gbps": round(alone_gbps, 3), "rounds": args.rounds,
@@ -1579,6 +1598,9 @@ def main():
                         help="kernels: KV heads in the cache, 8 / TP for one tensor-parallel rank's shard")
     parser.add_argument("--hash-depth", type=int, default=2,
                         help="save-restore: steps a save's digests may trail before they are collected")
+    parser.add_argument("--decode", choices=("reads", "attention"), default="reads",
+                        help="rotating-fp8: the decode beside the sessions reads its blocks, or attends over them "
+                             "(e4m3 with block scales, which the sessions' blocks then carry)")
     parser.add_argument("--rounds", type=int, default=4, help="rotating-fp8: rounds over the four sessions")
     parser.add_argument("--turns", type=int, default=6, help="turns: turns after the first save")
     parser.add_argument("--save-mode", choices=("staged", "direct"), default=None,

@@ -41,9 +41,12 @@ def make_caches(layers, num_blocks, *, block_size=16, heads=8, head_dim=128, dty
 
 
 def fill(plane, seed, *, kind=KIND_BF16, inv_scales=None, first_block=0, num_blocks=None, stream=None):
-    """Fill every span of blocks [first_block, first_block + num_blocks) of a registered plane."""
+    """Fill every span of the caches' blocks [first_block, first_block + num_blocks) of a registered plane; its
+    scales, if it has any, stay as they are."""
     import torch
     spans = plane.spans()
+    if getattr(plane, "scales", None) is not None:
+        spans = spans[:-1]
     device = next(iter(plane.caches.values())).device
     if num_blocks is None:
         num_blocks = min(plane._num_blocks(t) for t in plane.caches.values()) - first_block

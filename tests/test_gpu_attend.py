@@ -361,3 +361,26 @@ def test_the_same_call_gives_the_same_bits():
         first = layer.attend(query, tables, lengths, query_starts=starts)
         for _ in range(5):
             assert torch.equal(layer.attend(query, tables, lengths, query_starts=starts), first)
+
+
+@pytest.mark.parametrize("held", ["16-bit", "e4m3"])
+@pytest.mark.parametrize("count", [70, 130, 300])
+def test_many_sequences_of_every_length(count, held):
+    """More sequences than a wave looks at at a time (64), and than are cut evenly (256); a few long ones."""
+    rng = random.Random(count)
+    lengths = [rng.choice([0, 1, 15, 16, 40, 100]) for _ in range(count)]
+    for s, n in ((0, 2000), (count // 2, 1700), (count - 1, 2600)):
+        lengths[s] = n
+    blocks = sum(-(-n // 16) for n in lengths) + 1
+    layer, exact = make("kv_split", blocks, 16, 2, 32, E4M3 if held == "e4m3" else BF16, count)
+    tables = tables_for(lengths, 16, blocks, count)
+    lengths = torch.tensor(lengths, dtype=torch.int32)
+    query = made((count, 2, 32), BF16, 3)
+    out, lse = layer.attend(query.cuda(), tables.cuda(), lengths.cuda(), return_lse=True)
+    check(out, query, exact, tables, lengths, lse=lse)
+    # ragged: every fifth sequence has no row, every seventh three
+    added = [0 if s % 5 == 1 else 3 if s % 7 == 0 else 1 for s in range(count)]
+    starts = torch.tensor([sum(added[:s]) for s in range(count + 1)], dtype=torch.int32)
+    query = made((sum(added), 2, 32), BF16, 4)
+    out, lse = layer.attend(query.cuda(), tables.cuda(), lengths.cuda(), query_starts=starts.cuda(), return_lse=True)
+    check(out, query, exact, tables, lengths, starts, lse=lse)

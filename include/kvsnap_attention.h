@@ -31,6 +31,7 @@
  * read on the device and may change between replays of a captured launch.  A
  * table entry outside [0, blocks) names no block: nothing is written for it
  * and its tokens are seen by nobody; so are tokens past the table's width.
+ * A length counts up to 2^30, and a table names fewer tokens than that.
  */
 #ifndef KVSNAP_ATTENTION_H
 #define KVSNAP_ATTENTION_H
@@ -104,8 +105,8 @@ int kvsnap_append(const kvsnap_paged_layer* layer, const kvsnap_sequences* seque
                   int64_t tokens, int heads, int type, uintptr_t stream);
 
 /* Device bytes of scratch that kvsnap_attend needs over this layer (0: none);
- * ragged: whether it is given query_starts.  A max_length above what the
- * tables name counts as that. */
+ * ragged: whether it is given query_starts.  max_length: kvsnap_attend's, or
+ * table_width * block_size if that is less. */
 size_t kvsnap_attend_workspace_bytes(const kvsnap_paged_layer* layer, int64_t tokens, int n_seqs, int ragged, int heads,
                                      int64_t max_length, int64_t window);
 
@@ -114,7 +115,8 @@ size_t kvsnap_attend_workspace_bytes(const kvsnap_paged_layer* layer, int64_t to
  * `heads` heads (a multiple of the layer's, consecutive ones sharing a key
  * head) of type bf16 or fp16; a 16-bit cache is of the same type.  The row at
  * position p of its sequence sees tokens 0..p, with window > 0 the last
- * `window` of them; one that sees none has zeros (and a log sum of -inf).
+ * `window` of them; one that sees none, or scores of -inf alone, has
+ * zeros and a log sum of -inf.
  * Softmax, sums and products' sums are fp32; weights are rounded to 16 bits
  * before they meet the values (to two such terms for fp16 queries over an
  * e4m3 cache), and an e4m3 cache's values are exact in bf16.  lse, or NULL:

@@ -151,7 +151,8 @@ class PagedCache:
 
         Query heads are a multiple of the cache's; consecutive ones share a key head.  A row at position p sees the
         tokens 0 to p of its sequence, with ``window`` the last ``window`` of them, itself among them; a row that
-        sees none (a sequence of length 0) gets zeros.  Scores are ``softmax_scale`` (``width ** -0.5`` if None)
+        sees none (a sequence of length 0), or scores of -inf alone, gets zeros, and rows of ``out`` that are padding
+        stay as they are.  Scores are ``softmax_scale`` (``width ** -0.5`` if None)
         times the products; softmax and sums are fp32.  A 16-bit cache must have the query's type.
 
         ``max_length``, the longest sequence's length if the caller knows it (the tables' width if None), only shapes

@@ -593,7 +593,7 @@ __global__ __launch_bounds__(kTileWaves * 64, kD <= 128 ? 2 : 1) void attend_til
     // Threads side by side along a row, so that a wave's rows lie in one group of 16 tokens.
     constexpr int kBeside = kPieces <= 8 ? 8 : kPieces <= 16 ? 16 : 32;
     constexpr int kLoads = kTileTokens * kBeside / (kTileWaves * 64);
-        constexpr int kKeyRow = kD * 2 + 16, kValueRow = kD * 2 + (kD == 96 ? 0 : 64);
+    constexpr int kKeyRow = kD * 2 + 16, kValueRow = kD * 2 + (kD == 96 ? 0 : 64);
     constexpr int kStage = kTileTokens * (kKeyRow + kValueRow);
     constexpr uint32_t kNowhere = ~0u;
     __shared__ __attribute__((aligned(16))) char stage[2 * kStage];
@@ -791,7 +791,7 @@ __global__ __launch_bounds__(kTileWaves * 64, kD <= 128 ? 2 : 1) void attend_til
 #pragma unroll
         for (int i = 0; i < 16; ++i) sum[b][i] = 0;
     float top = -__builtin_inff(), total = 0;
-    const float factor = a.scale * kLog2e, slack = 8.0f / factor;
+    const float factor = a.scale * kLog2e, slack = __builtin_fminf(8.0f / factor, 1e30f);   // finite: -inf + slack is -inf
 
     if (thread < 6) odd[thread >> 1][thread & 1] = 0;
     int block = named_block(base);
@@ -1088,7 +1088,7 @@ __global__ __launch_bounds__(kJoinTileThreads) void join_tiles_kernel(Attend a) 
 
 // A tile of rows' tokens in parts: whole where there are tiles for two workgroups a CU.
 Split split_tiles(int64_t jobs, int64_t longest) {
-        constexpr int64_t least = 8 * kTileTokens, wanted = 1536, enough = 512;
+    constexpr int64_t least = 8 * kTileTokens, wanted = 1536, enough = 512;
     longest = std::max<int64_t>(longest, 1);
     if (jobs >= enough) return Split{1 << 29, 1};
     int64_t chunk = std::max(least, longest * jobs / wanted);
@@ -1192,8 +1192,8 @@ void launch_tiles(const Attend& a, unsigned grid, hipStream_t stream) {
     else launch_tiles_of<Q, kEight, true>(a, grid, stream);
 }
 
-unsigned checked_grid(int64_t groups) {
-    require(groups < (int64_t(1) << 31), "attend: too many rows for one launch");
+unsigned checked_grid(int64_t groups, int threads) {
+    require(groups * threads < (int64_t(1) << 32), "attend: too many rows for one launch");
     return static_cast<unsigned>(groups);
 }
 
@@ -1201,24 +1201,24 @@ template <typename Q>
 void launch_attend(const Attend& a, const Plan& plan, hipStream_t stream) {
     const bool eight = a.layer.type == KVSNAP_E4M3;
     if (plan.tile_slots) {
-        const unsigned grid = checked_grid(plan.tile_slots * a.tiles.chunks * a.layer.kv_heads);
+        const unsigned grid = checked_grid(plan.tile_slots * a.tiles.chunks * a.layer.kv_heads, kTileWaves * 64);
         if (eight) launch_tiles<Q, true>(a, grid, stream);
         else launch_tiles<Q, false>(a, grid, stream);
         check_launched("attend's tiles");
     }
-    const unsigned grid = checked_grid(plan.row_jobs);
+    const unsigned grid = checked_grid(plan.row_jobs, kWaves * 64);
     const unsigned lds = 4u * (kWaves * std::min(kHeadTile, a.group) * a.layer.width + 2 * kWaves * kHeadTile);
     if (eight) launch_rows<Q, true>(a, grid, lds, stream);
     else launch_rows<Q, false>(a, grid, lds, stream);
     check_launched("attend");
     if (plan.row_parts) {
-        hipLaunchKernelGGL(join_rows_kernel<Q>, dim3(checked_grid(int64_t(a.q.n_seqs) * a.heads)), dim3(kJoinThreads), 0,
-                           stream, a);
+        hipLaunchKernelGGL(join_rows_kernel<Q>, dim3(checked_grid(int64_t(a.q.n_seqs) * a.heads, kJoinThreads)),
+                           dim3(kJoinThreads), 0, stream, a);
         check_launched("attend's join");
     }
     if (plan.tile_parts) {
-        hipLaunchKernelGGL(join_tiles_kernel<Q>, dim3(checked_grid(int64_t(a.tokens) * a.heads)), dim3(kJoinTileThreads), 0,
-                           stream, a);
+        hipLaunchKernelGGL(join_tiles_kernel<Q>, dim3(checked_grid(int64_t(a.tokens) * a.heads, kJoinTileThreads)),
+                           dim3(kJoinTileThreads), 0, stream, a);
         check_launched("attend's join");
     }
 }

@@ -234,6 +234,12 @@ at::Tensor output(PyObject* object, const char* what, at::IntArrayRef sizes, con
     const at::Tensor& out = tensor(object, what);
     check_rows(out, what, sizes[0], sizes[1], sizes[2]);
     if (out.scalar_type() != like.scalar_type()) refuse(what, " must have the type of what it holds");
+    // Rows and heads apart from one another: the nearer axis by a head's width, the farther by all of the nearer.
+    const bool heads_inside = out.stride(1) <= out.stride(0) || out.size(0) <= 1;
+    const int inner = heads_inside && out.size(1) > 1 ? 1 : 0, outer = 1 - inner;
+    if (out.numel() > 0 && ((out.size(inner) > 1 && out.stride(inner) < out.size(2)) ||
+                            (out.size(outer) > 1 && out.stride(outer) < (out.size(inner) - 1) * out.stride(inner) + out.size(2))))
+        refuse(what, " must not overlap itself");
     return out;
 }
 

@@ -47,9 +47,12 @@ inline void check_layer(const kvsnap_paged_layer& layer) {
                 layer.block_stride * element % 16 == 0 && layer.token_stride * element % 16 == 0 &&
                 layer.head_stride * element % 16 == 0,
             "the cache's rows must be 16-byte aligned");
-    require(layer.block_stride >= 0 && layer.token_stride >= 0 && layer.head_stride >= 0 &&
-                layer.blocks * layer.block_stride * element < (int64_t(1) << 36),
-            "the cache's K or V must be under 64 GiB, its strides not negative");
+    // A block's start and its slots' places are added in 32 bits of 16 bytes, and 16 slots' places in 32 bits of bytes.
+    constexpr int64_t most = int64_t(1) << 36;
+    require(layer.block_stride >= 0 && layer.token_stride >= 0 && layer.head_stride >= 0 && layer.block_stride < most &&
+                layer.token_stride < (int64_t(1) << 26) &&
+                (layer.blocks * __int128(layer.block_stride) + layer.block_size * layer.token_stride) * element < most,
+            "the cache's K or V must be under 64 GiB, its strides not negative and a token's below 2^26");
     require((layer.scales != nullptr) == (layer.type == KVSNAP_E4M3), "an e4m3 cache has scales, another none");
 }
 

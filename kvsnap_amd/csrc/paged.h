@@ -61,8 +61,9 @@ __device__ __forceinline__ Rows rows_of(const kvsnap_sequences& q, int s, int to
     return Rows{first, max(end - first, 0)};
 }
 
-// Tokens of sequence s, and those of them that its table row can name.
-__device__ __forceinline__ int length_of(const kvsnap_sequences& q, int s) { return max(q.lengths[s], 0); }
+// Tokens of sequence s, at most 2^30 (no table names more) so that no position near them overflows, and those of them
+// that its table row can name.
+__device__ __forceinline__ int length_of(const kvsnap_sequences& q, int s) { return min(max(q.lengths[s], 0), 1 << 30); }
 __device__ __forceinline__ int named_of(const kvsnap_sequences& q, int length, int block_size) {
     const int64_t named = int64_t(q.table_width) * block_size;
     return length < named ? length : static_cast<int>(named);

@@ -365,3 +365,23 @@ def test_scales_that_a_plane_cannot_save_are_refused(scales, why):
         plane_with(Rows(**scales))
     with pytest.raises(ValueError, match="8-byte aligned"):
         plane_with(Rows(address=4100)).spans()
+
+
+@pytest.mark.parametrize("out,overlaps", [
+    (torch.zeros((4, 64)).as_strided((3, 2, 64), (64, 32, 1)), True),           # heads run into one another
+    (torch.zeros((1, 2, 64)).expand(3, 2, 64), True),
+    (torch.zeros((3, 1, 64)).expand(3, 2, 64), True),
+    (torch.zeros((2, 128)).as_strided((3, 2, 64), (64, 64, 1)), True),          # a row's second head is the next's first
+    (torch.zeros((2, 3, 64)).transpose(0, 1), False),
+    (torch.zeros((3, 2, 96))[..., :64], False),
+])
+def test_an_output_that_overlaps_itself_is_refused(out, overlaps):
+    with pytest.raises(ValueError, match="must not overlap itself" if overlaps else ON_CPU):
+        rotate(torch.zeros((3, 2, 64)), torch.zeros(3, dtype=torch.int64), torch.zeros((5, 32, 2)), out=out)
+
+
+@pytest.mark.parametrize("changes", [dict(token_stride=1 << 27), dict(block_stride=(1 << 60)),
+                                     dict(block_size=1 << 20, token_stride=1 << 20)])
+def test_the_c_entry_points_refuse_caches_whose_places_pass_32_bits(changes):
+    rc, message = c_attend(c_layer(**changes))
+    assert rc == -1 and "under 64 GiB" in message

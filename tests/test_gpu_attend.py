@@ -384,3 +384,32 @@ def test_many_sequences_of_every_length(count, held):
     query = made((sum(added), 2, 32), BF16, 4)
     out, lse = layer.attend(query.cuda(), tables.cuda(), lengths.cuda(), query_starts=starts.cuda(), return_lse=True)
     check(out, query, exact, tables, lengths, starts, lse=lse)
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+def test_a_scale_near_the_least_float_weighs_all_tokens_alike(rows):
+    layer, exact = make("vllm", 10, 16, 2, 64, BF16, 3)
+    lengths = torch.tensor([150], dtype=torch.int32)
+    tables = tables_for([150], 16, 10, 3)
+    starts = torch.tensor([0, rows], dtype=torch.int32)
+    query = made((rows, 4, 64), BF16, 4)
+    out, lse = layer.attend(query.cuda(), tables.cuda(), lengths.cuda(), query_starts=starts.cuda(), return_lse=True,
+                            softmax_scale=1.2e-38)
+    check(out, query, exact, tables, lengths, starts, lse=lse, scale=1.2e-38)
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+def test_a_length_that_no_table_names_sees_what_its_window_names(rows):
+    """Lengths up to int32's largest, far past the tables: with a window nobody sees a token, without one a row sees
+    all that is named, and every launch ends."""
+    layer, exact = make("vllm", 10, 16, 2, 64, BF16, 5)
+    named = tables_for([150], 16, 10, 5, spare=0)
+    starts = torch.tensor([0, rows], dtype=torch.int32).cuda()
+    query = made((rows, 4, 64), BF16, 6)
+    for length in (2 ** 30, 2 ** 31 - 1):
+        lengths = torch.tensor([length], dtype=torch.int32).cuda()
+        out, lse = layer.attend(query.cuda(), named.cuda(), lengths, query_starts=starts, window=100, return_lse=True)
+        assert not out.any() and lse.isneginf().all()
+        out = layer.attend(query.cuda(), named.cuda(), lengths, query_starts=starts)
+        # as the last rows of a sequence of all 160 named tokens and 1000 more, which no table names
+        check(out, query, exact, named, torch.tensor([1160], dtype=torch.int32), starts.cpu())

@@ -134,8 +134,13 @@ struct Parts {
 // Rows alone: how their tokens are cut into workgroups' jobs.
 struct RowJobs {
     int even;      // cut into equal parts, by the lengths that the sequences have, or `chunks` of `chunk` tiles each
-    int chunk, chunks, wanted;   // even: at least `chunk` tiles, for about `wanted` jobs
+    int chunk, chunks;
+    int wanted, room;   // even: at least `chunk` tiles, for up to `room` jobs, or about `wanted`
 };
+
+// Sequences that a wave goes over, 64 at a time, to cut their tokens evenly; more have parts of one length, by the
+// longest.
+constexpr int kEvenSeqs = 256;
 
 struct Attend {
     kvsnap_paged_layer layer;
@@ -197,23 +202,19 @@ __device__ __forceinline__ int row_tiles(const Attend& a, int sequence) {
     return max((sight.high - (sight.low & ~(kTile - 1)) + kTile - 1) / kTile, 1);
 }
 
-__device__ __forceinline__ int wave_sum(int x) {
-#pragma unroll
-    for (int step = 1; step < 64; step <<= 1) x += __shfl_xor(x, step);
-    return __builtin_amdgcn_readfirstlane(x);
+// Sums of the wave's values up to each lane's, by moves between lanes that need no LDS.
+__device__ __forceinline__ int wave_scan(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);     // from 1, 2, 4 and 8 lanes below, of 16
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);     // lane 15 of 16 to the next 16
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);     // lane 31 to the upper half
+    return x;
 }
+__device__ __forceinline__ int wave_sum(int x) { return __builtin_amdgcn_readlane(wave_scan(x), 63); }
 
-// Where even parts are cut: all sequences' tiles over the jobs wanted, in whole turns of a workgroup's waves.
-__device__ __forceinline__ int even_chunk(const Attend& a, int head_groups) {
-    const int lane = __lane_id(), in_turn = kWaves / a.beside;
-    int64_t all = 0;
-    for (int s = 0; s < a.q.n_seqs; s += 64) all += wave_sum(s + lane < a.q.n_seqs ? row_tiles(a, s + lane) : 0);
-    const int chunk = static_cast<int>(max(int64_t(a.rows.chunk), (all * head_groups + a.rows.wanted - 1) / a.rows.wanted));
-    return (chunk + in_turn - 1) / in_turn * in_turn;
-}
-
-// The sequence whose jobs hold `job`, and its parts.  A wave goes over 64 sequences at a time, their jobs summed from
-// the first on.
+// The sequence whose jobs hold `job`, and its parts.
 __device__ __forceinline__ RowJob row_job(const Attend& a, int64_t job, int head_groups) {
     if (!a.rows.even) {
         const int sequence = static_cast<int>(job / (a.rows.chunks * head_groups));
@@ -223,23 +224,43 @@ __device__ __forceinline__ RowJob row_job(const Attend& a, int64_t job, int head
         return RowJob{tiles ? sequence : -1, rest % head_groups, rest / head_groups,
                       min((tiles + a.rows.chunk - 1) / a.rows.chunk, a.rows.chunks), a.rows.chunk, first};
     }
-    const int lane = __lane_id(), chunk = even_chunk(a, head_groups);
-    int64_t before = 0;
-    for (int s = 0; s < a.q.n_seqs; s += 64) {
-        const int mine = s + lane < a.q.n_seqs ? (row_tiles(a, s + lane) + chunk - 1) / chunk : 0;
-        int up_to = mine;
+    // Even parts: all sequences' tiles over the jobs wanted, in whole turns of a workgroup's waves.  A lane holds the
+    // tiles of every 64th sequence.
+    constexpr int kTurns = kEvenSeqs / 64;
+    const int lane = __lane_id(), in_turn = kWaves / a.beside;
+    int tiles[kTurns];
+    int64_t all = 0;
 #pragma unroll
-        for (int step = 1; step < 64; step <<= 1) {
-            const int other = __shfl_up(up_to, step);
-            up_to += lane >= step ? other : 0;
-        }
+    for (int i = 0; i < kTurns; ++i)        // (their sum in 32 bits: what is past 2^29 tokens goes to the last part)
+        tiles[i] = 64 * i + lane < a.q.n_seqs ? min(row_tiles(a, 64 * i + lane), 1 << 24) : 0;
+#pragma unroll
+    for (int i = 0; i < kTurns; ++i)
+        if (64 * i < a.q.n_seqs) all += wave_sum(tiles[i]);
+    const auto chunk_for = [&](int jobs) {
+        const int chunk = static_cast<int>(max(int64_t(a.rows.chunk), (all * head_groups + jobs - 1) / jobs));
+        return (chunk + in_turn - 1) / in_turn * in_turn;
+    };
+    // As many jobs as there is room for, if the sequences' last parts leave it so, or somewhat fewer.
+    int chunk = chunk_for(a.rows.room);
+    if (a.rows.room > a.rows.wanted) {
+        int64_t jobs = 0;
+#pragma unroll
+        for (int i = 0; i < kTurns; ++i)
+            if (64 * i < a.q.n_seqs) jobs += wave_sum((tiles[i] + chunk - 1) / chunk);
+        if (jobs * head_groups > a.rows.room) chunk = chunk_for(a.rows.wanted);
+    }
+    int64_t before = 0;
+#pragma unroll
+    for (int i = 0; i < kTurns; ++i) {
+        if (64 * i >= a.q.n_seqs) break;
+        const int mine = (tiles[i] + chunk - 1) / chunk, up_to = wave_scan(mine);
         const uint64_t holds = __ballot(before + int64_t(up_to) * head_groups > job);
         if (holds) {
             const int at = __builtin_ctzll(holds);
             const int parts = __builtin_amdgcn_readlane(mine, at);
             const int64_t first = before + int64_t(__builtin_amdgcn_readlane(up_to, at) - parts) * head_groups;
             const int rest = static_cast<int>(job - first);
-            return RowJob{parts ? s + at : -1, rest % head_groups, rest / head_groups, parts, chunk, first};
+            return RowJob{parts ? 64 * i + at : -1, rest % head_groups, rest / head_groups, parts, chunk, first};
         }
         before += int64_t(__builtin_amdgcn_readlane(up_to, 63)) * head_groups;
     }
@@ -1109,14 +1130,13 @@ struct Plan {
 // of up to 8k tokens in e4m3 (322 MB) take 76 us with 8 heads beside, 79 with 4 and 104 with one.  Few rows are better
 // off with all the waves on one head: the parts are joined in LDS, and one of 32k tokens takes 24.6 us, not 30.9.
 constexpr int kFewHeads = 16;
-// Jobs that the sequences' tokens are cut into: in e4m3 what the chip holds at once, so that all end together (76 us
-// with 450, 88 with 600); a 16-bit cache's jobs are longer, and twice as many are better (135 us, 152 with 500).
-constexpr int kJobsE4m3 = 450, kJobs16 = 1000;
+// Jobs that the sequences' tokens are cut into: in e4m3 at most what the chip holds at once, so that all end together:
+// 512 where the sequences' last parts allow it (one of 32k tokens takes 22.0 us, 24.8 with 450), else about 450 (the 64
+// ragged ones take 76 us, 87 with 512 asked for and some 530 made).  A 16-bit cache's jobs are longer, and twice as many
+// are better (135 us, 152 with 500).
+constexpr int kRoomE4m3 = 512, kJobsE4m3 = 450, kJobs16 = 1000;
 // Tiles of a wave up to which a row is not cut, the join being 4 to 6 us, and of a part at least.
 constexpr int kWholeTurns = 5, kLeastTurns = 2;
-// Sequences that a wave goes over, 64 at a time, to cut their tokens evenly; more have parts of one length, by the
-// longest.
-constexpr int kEvenSeqs = 256;
 
 Plan plan_of(int64_t tokens, int n_seqs, bool ragged, int heads, int kv_heads, bool eight, int64_t max_length,
              int64_t window) {
@@ -1131,13 +1151,13 @@ Plan plan_of(int64_t tokens, int n_seqs, bool ragged, int heads, int kv_heads, b
     const int64_t tiles = std::max<int64_t>((longest + kTile - 1) / kTile + 1, 1);
     const int64_t in_turn = kWaves / plan.beside;
     const int64_t least = kLeastTurns * in_turn, whole = kWholeTurns * in_turn;
-    const int wanted = eight ? kJobsE4m3 : kJobs16;
-    plan.rows = RowJobs{0, 1 << 24, 1, wanted};
+    const int wanted = eight ? kJobsE4m3 : kJobs16, room = eight ? kRoomE4m3 : kJobs16;
+    plan.rows = RowJobs{0, 1 << 24, 1, wanted, room};
     plan.row_jobs = row_jobs;
     if (tiles > whole && n_seqs <= kEvenSeqs) {
         plan.rows.even = 1;
         plan.rows.chunk = static_cast<int>(least);
-        plan.row_jobs += wanted;
+        plan.row_jobs += room;
         plan.row_parts = plan.row_jobs * plan.beside * plan.slots;
     } else if (tiles > whole) {
         plan.rows.chunk = static_cast<int>(std::min<int64_t>(std::max(least, tiles * row_jobs / (2 * wanted)), 1 << 24));

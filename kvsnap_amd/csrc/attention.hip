@@ -131,14 +131,18 @@ struct Parts {
     float *sums, *totals;
 };
 
-// Rows alone: how their tokens are cut into workgroups' jobs.
+// Rows alone, and tiles of rows: how their tokens are cut into workgroups' jobs.
 struct RowJobs {
     int even;      // cut into equal parts, by the lengths that the sequences have, or `chunks` of `chunk` tiles each
     int chunk, chunks;
-    int wanted, room;   // even: at least `chunk` tiles, for up to `room` jobs, or about `wanted`
+    int room, fitted;   // even: at least `chunk` tiles, for about `room` jobs, or no more than those
 };
 
-// Sequences that a wave goes over, 64 at a time, to cut their tokens evenly; more have parts of one length, by the
+struct TileJobs {
+    int even, room;     // cut into parts for up to `room` jobs more than there are tiles, or whole
+};
+
+// Sequences that a wave goes over, 64 at a time, to cut their rows' tokens evenly; more have parts of one length, by the
 // longest.
 constexpr int kEvenSeqs = 256;
 
@@ -153,9 +157,11 @@ struct Attend {
     float scale;
     int window;                // 0: none
     RowJobs rows;
-    Split tiles;               // of a tile of rows
-    Parts row_parts, tile_parts;  // [job, beside, heads of a tile], and [row, head, part]
+    TileJobs tiles;
+    Parts row_parts, tile_parts;  // [job, beside, heads of a tile], and [job, rows of a tile]
     int2* row_info;               // [sequence, heads' group]: the first job and the parts of rows alone
+    int2* tile_info;              // [sequence, 2]: the first job of its tiles and their parts, tokens of a part and tiles
+    int tile_jobs;                // that there is room for
     int head_tiles;            // of 16 heads, of a key head's
     int beside;                // key heads that a workgroup's waves take side by side
     int slots;                 // heads of a tile, at most
@@ -214,6 +220,54 @@ __device__ __forceinline__ int wave_scan(int x) {
 }
 __device__ __forceinline__ int wave_sum(int x) { return __builtin_amdgcn_readlane(wave_scan(x), 63); }
 
+__device__ __forceinline__ int64_t wave_sum64(int64_t x) {     // of values from 0 to 2^40
+    return (int64_t(wave_sum(static_cast<int>(x >> 16))) << 16) + wave_sum(static_cast<int>(x & 0xffff));
+}
+
+// The sequence whose jobs hold `job`: its first job, its parts, and how long one is.
+struct Cut {
+    int sequence, parts, chunk;
+    int64_t first;
+};
+
+// Work cut evenly over `room` jobs.  A lane holds the `units` of every 64th sequence (0: none of these jobs), `times`
+// times over; a sequence has `each` jobs for every part and time.  Parts are whole multiples of `step` units, `least` at
+// the least: `all` over `room`, or up to most_eighths / 8 of that, the shortest tried with which the jobs come out as no
+// more than `room`.
+template <int kTurns>
+__device__ __forceinline__ Cut even_cut(int n_seqs, int64_t job, const int (&units)[kTurns], const int (&times)[kTurns],
+                                        int each, int least, int step, int room, int most_eighths) {
+    int64_t mine_of_all = 0;
+#pragma unroll
+    for (int i = 0; i < kTurns; ++i) mine_of_all += int64_t(units[i]) * times[i];
+    const int64_t all = wave_sum64(mine_of_all);
+    int chunk = 0;
+#pragma unroll 1
+    for (int eighths = 8; eighths <= most_eighths; ++eighths) {
+        const int64_t share = (all * each * eighths + 8 * room - 1) / (8 * room);
+        chunk = (static_cast<int>(max(int64_t(least), share)) + step - 1) / step * step;
+        if (eighths == most_eighths) break;
+        int jobs = 0;
+#pragma unroll
+        for (int i = 0; i < kTurns; ++i) jobs += (units[i] + chunk - 1) / chunk * times[i];
+        if (int64_t(wave_sum(jobs)) * each <= room) break;
+    }
+    int64_t before = 0;
+#pragma unroll
+    for (int i = 0; i < kTurns; ++i) {
+        if (64 * i >= n_seqs) break;
+        const int parts = (units[i] + chunk - 1) / chunk, mine = parts * times[i], up_to = wave_scan(mine);
+        const uint64_t holds = __ballot(before + int64_t(up_to) * each > job);
+        if (holds) {
+            const int at = __builtin_ctzll(holds);
+            const int upto_before = __builtin_amdgcn_readlane(up_to, at) - __builtin_amdgcn_readlane(mine, at);
+            return Cut{64 * i + at, __builtin_amdgcn_readlane(parts, at), chunk, before + int64_t(upto_before) * each};
+        }
+        before += int64_t(__builtin_amdgcn_readlane(up_to, 63)) * each;
+    }
+    return Cut{-1, 0, 1, 0};
+}
+
 // The sequence whose jobs hold `job`, and its parts.
 __device__ __forceinline__ RowJob row_job(const Attend& a, int64_t job, int head_groups) {
     if (!a.rows.even) {
@@ -224,47 +278,18 @@ __device__ __forceinline__ RowJob row_job(const Attend& a, int64_t job, int head
         return RowJob{tiles ? sequence : -1, rest % head_groups, rest / head_groups,
                       min((tiles + a.rows.chunk - 1) / a.rows.chunk, a.rows.chunks), a.rows.chunk, first};
     }
-    // Even parts: all sequences' tiles over the jobs wanted, in whole turns of a workgroup's waves.  A lane holds the
-    // tiles of every 64th sequence.
-    constexpr int kTurns = kEvenSeqs / 64;
-    const int lane = __lane_id(), in_turn = kWaves / a.beside;
-    int tiles[kTurns];
-    int64_t all = 0;
+    const int lane = __lane_id();
+    int tiles[kEvenSeqs / 64], once[kEvenSeqs / 64];
 #pragma unroll
-    for (int i = 0; i < kTurns; ++i)        // (their sum in 32 bits: what is past 2^29 tokens goes to the last part)
+    for (int i = 0; i < kEvenSeqs / 64; ++i) {      // what is past 2^29 tokens goes to a row's last part
         tiles[i] = 64 * i + lane < a.q.n_seqs ? min(row_tiles(a, 64 * i + lane), 1 << 24) : 0;
-#pragma unroll
-    for (int i = 0; i < kTurns; ++i)
-        if (64 * i < a.q.n_seqs) all += wave_sum(tiles[i]);
-    const auto chunk_for = [&](int jobs) {
-        const int chunk = static_cast<int>(max(int64_t(a.rows.chunk), (all * head_groups + jobs - 1) / jobs));
-        return (chunk + in_turn - 1) / in_turn * in_turn;
-    };
-    // As many jobs as there is room for, if the sequences' last parts leave it so, or somewhat fewer.
-    int chunk = chunk_for(a.rows.room);
-    if (a.rows.room > a.rows.wanted) {
-        int64_t jobs = 0;
-#pragma unroll
-        for (int i = 0; i < kTurns; ++i)
-            if (64 * i < a.q.n_seqs) jobs += wave_sum((tiles[i] + chunk - 1) / chunk);
-        if (jobs * head_groups > a.rows.room) chunk = chunk_for(a.rows.wanted);
+        once[i] = 1;
     }
-    int64_t before = 0;
-#pragma unroll
-    for (int i = 0; i < kTurns; ++i) {
-        if (64 * i >= a.q.n_seqs) break;
-        const int mine = (tiles[i] + chunk - 1) / chunk, up_to = wave_scan(mine);
-        const uint64_t holds = __ballot(before + int64_t(up_to) * head_groups > job);
-        if (holds) {
-            const int at = __builtin_ctzll(holds);
-            const int parts = __builtin_amdgcn_readlane(mine, at);
-            const int64_t first = before + int64_t(__builtin_amdgcn_readlane(up_to, at) - parts) * head_groups;
-            const int rest = static_cast<int>(job - first);
-            return RowJob{parts ? 64 * i + at : -1, rest % head_groups, rest / head_groups, parts, chunk, first};
-        }
-        before += int64_t(__builtin_amdgcn_readlane(up_to, 63)) * head_groups;
-    }
-    return RowJob{-1, 0, 0, 0, 0, 0};
+    // In whole turns of a workgroup's waves.
+    const Cut cut = even_cut(a.q.n_seqs, job, tiles, once, head_groups, a.rows.chunk, kWaves / a.beside, a.rows.room,
+                             a.rows.fitted ? 12 : 8);
+    const int rest = static_cast<int>(job - cut.first);
+    return RowJob{cut.sequence, rest % head_groups, rest / head_groups, cut.parts, cut.chunk, cut.first};
 }
 
 // One wave's loads of a tile: K's rows for the first product and V's for the second.
@@ -278,10 +303,16 @@ struct Tile {
     float k_scale[2], v_scale[2][4];                        // e4m3 only
 };
 
-// A row's heads of one key head over one part of its tokens, a workgroup of four waves that take tiles in turn.
+// A row's heads of `beside` key heads over one part of its tokens, a workgroup of eight waves; those of one key head take
+// its tiles of 32 tokens in turn.
 //
 // Bound by reading K and V once: 16 query rows of a product are used for `group` heads, a quarter of them for groups
-// of four, and the matrix cores still wait for memory.
+// of four, and the matrix cores still wait for memory.  Loads go straight to the registers that the products take, as no
+// wave shares them; sixteen waves a CU are what hides their latency (a tile's loads ahead of their use, at eight waves,
+// measured the same).  64 ragged rows over 322 MB of e4m3 take 67 us, 4.8 TB/s where a plain read of as much reaches 6.6,
+// and 6 for the join; what is missing is the start, four loads that follow from one another (length, table, rows), and
+// the last workgroups' end.  Loads that keep out of the caches (nontemporal) are 5 % faster there and up to 45 % slower
+// where a cache fits what the chip's does.
 template <typename Q, bool kEight, int kJ, bool kWhole, bool kExact>
 __global__ __launch_bounds__(kWaves * 64, kEight && kJ <= 8 ? 4 : 2) void attend_row_kernel(Attend a) {
     using T = typename Shape<Q, kEight>::T;
@@ -583,11 +614,64 @@ __global__ __launch_bounds__(kWaves * 64, kEight && kJ <= 8 ? 4 : 2) void attend
 constexpr int kTileRows = 128;    // rows of a workgroup: (token, head) pairs that share a key head, heads fastest
 constexpr int kTileWaves = 4;     // 32 rows each, the columns of a product
 constexpr int kTileTokens = 64;   // tokens staged at a time
+constexpr int kTileSeqs = 512;    // sequences at most where tiles are cut
+constexpr int kLeastStages = 8;   // of 64 tokens, of a part
 
 // The tile of a sequence's rows that starts at pair `first`: the tokens of its first and last pair.
 __device__ __forceinline__ Sight tile_sight(const Attend& a, int sequence, const Rows& rows, int first) {
     const int last = min(first + kTileRows, rows.count * a.group) - 1;
     return sight_of(a, sequence, rows, a.group_size.divide(first), a.group_size.divide(last));
+}
+
+// A workgroup's job: a part of what a tile of a sequence's rows sees, for a key head.
+struct TileJob {
+    int sequence, kv_head, part;
+    int64_t pair;       // the tile's first
+    Split split;
+};
+
+// Tiles whole.  Sequence s has slots from query_starts[s] * group / 128 + s on: n rows have at most n * group / 128 + 1
+// tiles.  Later ones see more tokens: they go first.
+__device__ __forceinline__ TileJob whole_tile_job(const Attend& a, uint32_t job, uint32_t jobs) {
+    const auto slots = [&](int s) {
+        return int64_t(min(max(a.q.query_starts[s], 0), a.tokens)) * a.group / kTileRows + s;
+    };
+    const int64_t slot = (jobs - 1 - job) / a.layer.kv_heads;
+    const int sequence = find_sequence(a.q.n_seqs, slot, slots);
+    return TileJob{sequence, static_cast<int>(job % a.layer.kv_heads), 0, (slot - slots(sequence)) * kTileRows,
+                   Split{1 << 29, 1}};
+}
+
+// Tiles in parts, by the lengths that the sequences have: a sequence's tiles are cut as its last is.  The workgroups of
+// one key head's tiles follow one another by the number of key heads.
+__device__ __forceinline__ TileJob even_tile_job(const Attend& a, uint32_t job) {
+    constexpr int kTurns = kTileSeqs / 64;
+    const int lane = __lane_id(), kv_heads = a.layer.kv_heads;
+    int stages[kTurns], tiles[kTurns];
+#pragma unroll
+    for (int i = 0; i < kTurns; ++i) {
+        const int s = 64 * i + lane;
+        stages[i] = tiles[i] = 0;
+        if (s >= a.q.n_seqs) continue;
+        const Rows rows = rows_of(a.q, s, a.tokens);
+        if (rows.count < 2) continue;
+        tiles[i] = (rows.count * a.group + kTileRows - 1) / kTileRows;
+        const Sight sight = tile_sight(a, s, rows, (tiles[i] - 1) * kTileRows);
+        stages[i] = min(max((sight.high - (sight.low & ~(kTileTokens - 1)) + kTileTokens - 1) / kTileTokens, 1), 1 << 23);
+    }
+    const Cut cut = even_cut(a.q.n_seqs, job, stages, tiles, kv_heads, kLeastStages, 1, a.tiles.room, 12);
+    if (cut.sequence < 0) return TileJob{-1, 0, 0, 0, Split{1, 1}};
+    int tiles_of = 0;
+#pragma unroll
+    for (int i = 0; i < kTurns; ++i)
+        if (cut.sequence >> 6 == i) tiles_of = __builtin_amdgcn_readlane(tiles[i], cut.sequence & 63);
+    const int rest = static_cast<int>(job - cut.first), time = rest / kv_heads;
+    const Split split{cut.chunk * kTileTokens, cut.parts};
+    if (rest == 0 && threadIdx.x == 0) {
+        a.tile_info[2 * cut.sequence] = int2{static_cast<int>(cut.first), cut.parts};
+        a.tile_info[2 * cut.sequence + 1] = int2{split.chunk, tiles_of};
+    }
+    return TileJob{cut.sequence, rest % kv_heads, time / tiles_of, int64_t(time % tiles_of) * kTileRows, split};
 }
 
 // Whether a pair of 16-bit values holds one that is not finite (`ones`: the type's exponent bits, twice).
@@ -603,6 +687,13 @@ __device__ __forceinline__ uint32_t not_finite(uint32_t word) {
 // K's rows are 16 bytes longer than the values (an odd number of 16-byte pieces: 16-byte reads down a column of rows
 // meet every bank); V's are 64 or 192 bytes past a multiple of 256, so that the 64 bytes of four rows that half a wave's
 // transposing read takes lie side by side over the banks.  No read waits for a bank.
+//
+// An 8k prompt of 32 heads over 8 of 128 in bf16 takes 630 us, 870 TFLOP/s of the products that its mask leaves, where a
+// large plain product reaches 1280 on this card.  A stage costs a wave 1024 cycles of products and about 1100 of vector
+// instructions (32 scores a lane: a multiplication, an exponential, a sum, half a rounding, half a maximum), and the two
+// waves of a SIMD overlap little of the two.  Tried and slower: the next stage's scores between this stage's
+// exponentials (1004 us at 256 registers, and 476 against 395 at width 64, where nothing spills), and higher priority
+// for waves in their products (662).
 template <typename Q, bool kEight, int kD, bool kWhole>
 __global__ __launch_bounds__(kTileWaves * 64, kD <= 128 ? 2 : 1) void attend_tile_kernel(Attend a) {
     using T = typename Shape<Q, kEight>::T;
@@ -620,26 +711,17 @@ __global__ __launch_bounds__(kTileWaves * 64, kD <= 128 ? 2 : 1) void attend_til
     __shared__ __attribute__((aligned(16))) char stage[2 * kStage];
     __shared__ uint32_t odd[3][2];                          // tokens with a value that is not finite, by turns
 
-    const int kv_heads = a.layer.kv_heads;
-    uint32_t job = blockIdx.x;
-    const int kv_head = job % kv_heads;
-    job /= kv_heads;
-    const int part = job % a.tiles.chunks;
-    // Later tiles see more tokens: they go first.
-    const int64_t slot_of_all = gridDim.x / kv_heads / a.tiles.chunks - 1 - job / a.tiles.chunks;
-    // Sequence s has slots from query_starts[s] * group / 128 + s on: n rows have at most n * group / 128 + 1 tiles.
-    const auto slots = [&](int s) {
-        return int64_t(min(max(a.q.query_starts[s], 0), a.tokens)) * a.group / kTileRows + s;
-    };
-    const int sequence = find_sequence(a.q.n_seqs, slot_of_all, slots);
+    const TileJob job = a.tiles.even ? even_tile_job(a, blockIdx.x) : whole_tile_job(a, blockIdx.x, gridDim.x);
+    if (job.sequence < 0) return;
+    const auto same = [](int x) { return __builtin_amdgcn_readfirstlane(x); };      // kept in scalar registers
+    const int sequence = same(job.sequence), kv_head = same(job.kv_head), part = same(job.part);
     const Rows rows = rows_of(a.q, sequence, a.tokens);
-    if (rows.count < 2) return;                             // none, or a row alone
-    const int64_t first_pair = (slot_of_all - slots(sequence)) * kTileRows;
     const int pairs = rows.count * a.group;
-    if (first_pair < 0 || first_pair >= pairs) return;
-    const int pair0 = static_cast<int>(first_pair);
+    if (rows.count < 2 || job.pair < 0 || job.pair >= pairs) return;    // no rows, or a row alone
+    const int pair0 = same(static_cast<int>(job.pair));
+    const Split split{same(job.split.chunk), same(job.split.chunks)};
     const Sight sight = tile_sight(a, sequence, rows, pair0);
-    const int parts = parts_of<kTileTokens>(a.tiles, sight);
+    const int parts = parts_of<kTileTokens>(split, sight);
     if (part >= max(parts, 1)) return;
 
     const int width = a.layer.width;
@@ -677,8 +759,8 @@ __global__ __launch_bounds__(kTileWaves * 64, kD <= 128 ? 2 : 1) void attend_til
         }
     }
 
-    const int base = (sight.low & ~(kTileTokens - 1)) + part * a.tiles.chunk;
-    const int stop = part == a.tiles.chunks - 1 ? sight.high : min(sight.high, base + a.tiles.chunk);
+    const int base = (sight.low & ~(kTileTokens - 1)) + part * split.chunk;
+    const int stop = part == split.chunks - 1 ? sight.high : min(sight.high, base + split.chunk);
     const int32_t* const table = a.q.block_tables + sequence * a.q.table_stride;
     const char* const keys = static_cast<const char*>(a.layer.key) + kv_head * a.layer.head_stride * kBytes;
     const char* const values = static_cast<const char*>(a.layer.value) + kv_head * a.layer.head_stride * kBytes;
@@ -984,7 +1066,7 @@ __global__ __launch_bounds__(kTileWaves * 64, kD <= 128 ? 2 : 1) void attend_til
     if (!real) return;
     const int64_t index = row * a.heads + head;
     const float share = parts > 1 ? 1.0f : over(total);
-    const int64_t at_part = index * a.tiles.chunks + part;
+    const int64_t at_part = int64_t(blockIdx.x) * kTileRows + pair - pair0;
     float* const sums = a.tile_parts.sums + at_part * width;
     Q* const out = static_cast<Q*>(a.out) + row * a.out_token_stride + head * a.out_head_stride;
 #pragma unroll
@@ -1098,30 +1180,27 @@ __global__ __launch_bounds__(kJoinTileThreads) void join_tiles_kernel(Attend a) 
     const Rows rows = rows_of(a.q, sequence, a.tokens);
     const int mine = row - rows.first;
     if (mine < 0 || mine >= rows.count || rows.count == 1) return;
-    const int pair = mine * a.group + (head - a.group_size.divide(head) * a.group);
-    const int parts = parts_of<kTileTokens>(a.tiles, tile_sight(a, sequence, rows, pair / kTileRows * kTileRows));
-    if (parts < 2) return;
-    const int64_t first = (int64_t(row) * a.heads + head) * a.tiles.chunks;
-    join<Q, kJoinTileThreads>(a, a.tile_parts.sums + first * a.layer.width, a.tile_parts.totals + first * 2, 1, parts, row, head);
+    const int kv_head = a.group_size.divide(head), pair = mine * a.group + (head - kv_head * a.group);
+    const int tile = pair / kTileRows;
+    const int2 info = a.tile_info[2 * sequence], about = a.tile_info[2 * sequence + 1];
+    const int64_t jobs = int64_t(about.y) * a.layer.kv_heads;           // of a part
+    // Row starts that do not rise may leave a sequence without a workgroup, and its entry unwritten.
+    if (info.x < 0 || info.y < 2 || about.x < 1 || tile >= about.y || info.x + jobs * info.y > a.tile_jobs) return;
+    const int parts = parts_of<kTileTokens>(Split{about.x, info.y}, tile_sight(a, sequence, rows, tile * kTileRows));
+    if (parts < 2) return;                                  // written by the one workgroup that took it
+    const int64_t first = (info.x + int64_t(tile) * a.layer.kv_heads + kv_head) * kTileRows + pair % kTileRows;
+    join<Q, kJoinTileThreads>(a, a.tile_parts.sums + first * a.layer.width, a.tile_parts.totals + first * 2,
+                              jobs * kTileRows, parts, row, head);
 }
 
 // ----------------------------------------------------------------- launches
 
-// A tile of rows' tokens in parts: whole where there are tiles for two workgroups a CU.
-Split split_tiles(int64_t jobs, int64_t longest) {
-    constexpr int64_t least = 8 * kTileTokens, wanted = 1536, enough = 512;
-    longest = std::max<int64_t>(longest, 1);
-    if (jobs >= enough) return Split{1 << 29, 1};
-    int64_t chunk = std::max(least, longest * jobs / wanted);
-    chunk = std::min<int64_t>((chunk + kTileTokens - 1) / kTileTokens * kTileTokens, 1 << 29);
-    return Split{static_cast<int>(chunk), static_cast<int>((longest + kTileTokens - 1 + chunk - 1) / chunk)};
-}
-
 struct Plan {
     RowJobs rows;
-    Split tiles;
+    TileJobs tiles;
     int beside, slots;
-    int64_t row_infos = 0, row_jobs, tile_slots, row_parts, tile_parts;  // parts: of all heads, 0 where rows are whole
+    // Parts: of all heads, 0 where rows are whole.
+    int64_t row_infos = 0, tile_infos = 0, row_jobs, tile_jobs, row_parts, tile_parts;
 };
 
 // How the rows alone are cut, as measured with 32 query heads, 8 key heads of 128 and blocks of 16 tokens.
@@ -1130,17 +1209,22 @@ struct Plan {
 // of up to 8k tokens in e4m3 (322 MB) take 76 us with 8 heads beside, 79 with 4 and 104 with one.  Few rows are better
 // off with all the waves on one head: the parts are joined in LDS, and one of 32k tokens takes 24.6 us, not 30.9.
 constexpr int kFewHeads = 16;
-// Jobs that the sequences' tokens are cut into: in e4m3 at most what the chip holds at once, so that all end together:
-// 512 where the sequences' last parts allow it (one of 32k tokens takes 22.0 us, 24.8 with 450), else about 450 (the 64
-// ragged ones take 76 us, 87 with 512 asked for and some 530 made).  A 16-bit cache's jobs are longer, and twice as many
-// are better (135 us, 152 with 500).
-constexpr int kRoomE4m3 = 512, kJobsE4m3 = 450, kJobs16 = 1000;
+// Jobs that the sequences' tokens are cut into: in e4m3 no more than the chip holds at once (one row over 32k tokens:
+// 22.0 us; 24.8 with 450 asked for; the 64 ragged ones 76 us, 87 with 512 asked for and some 530 made).  A 16-bit cache's
+// jobs are longer, and about twice as many are better (135 us, 152 with 500; 141 with no more than 1000).
+constexpr int kRoomE4m3 = 512, kRoom16 = 1000;
 // Tiles of a wave up to which a row is not cut, the join being 4 to 6 us, and of a part at least.
 constexpr int kWholeTurns = 5, kLeastTurns = 2;
 
+// Tiles whose jobs are fewer than the chip holds at once (two workgroups a CU) are cut into no more than it holds, where
+// that comes out: 12 sequences of up to 7700 tokens with 693 rows (16 heads over 8 of 128, e4m3) take 75 us; parts of one
+// length by the longest sequence's, as for three rounds, took 87, the last round being nearly empty.
+constexpr int kTileRoom = 512;
+static_assert(kTileRoom <= kTileSeqs, "tiles that are cut are of fewer sequences than a wave goes over");
+
 Plan plan_of(int64_t tokens, int n_seqs, bool ragged, int heads, int kv_heads, bool eight, int64_t max_length,
              int64_t window) {
-    const int64_t longest = window > 0 ? std::min(window, max_length) : max_length;
+    int64_t longest = window > 0 ? std::min(window, max_length) : max_length;
     const int64_t group = heads / kv_heads, head_tiles = (group + kHeadTile - 1) / kHeadTile;
     Plan plan{};
     plan.beside = 1;
@@ -1151,8 +1235,8 @@ Plan plan_of(int64_t tokens, int n_seqs, bool ragged, int heads, int kv_heads, b
     const int64_t tiles = std::max<int64_t>((longest + kTile - 1) / kTile + 1, 1);
     const int64_t in_turn = kWaves / plan.beside;
     const int64_t least = kLeastTurns * in_turn, whole = kWholeTurns * in_turn;
-    const int wanted = eight ? kJobsE4m3 : kJobs16, room = eight ? kRoomE4m3 : kJobs16;
-    plan.rows = RowJobs{0, 1 << 24, 1, wanted, room};
+    const int room = eight ? kRoomE4m3 : kRoom16;
+    plan.rows = RowJobs{0, 1 << 24, 1, room, eight};
     plan.row_jobs = row_jobs;
     if (tiles > whole && n_seqs <= kEvenSeqs) {
         plan.rows.even = 1;
@@ -1160,25 +1244,29 @@ Plan plan_of(int64_t tokens, int n_seqs, bool ragged, int heads, int kv_heads, b
         plan.row_jobs += room;
         plan.row_parts = plan.row_jobs * plan.beside * plan.slots;
     } else if (tiles > whole) {
-        plan.rows.chunk = static_cast<int>(std::min<int64_t>(std::max(least, tiles * row_jobs / (2 * wanted)), 1 << 24));
+        plan.rows.chunk = static_cast<int>(std::min<int64_t>(std::max(least, tiles * row_jobs / (2 * room)), 1 << 24));
         plan.rows.chunks = static_cast<int>((tiles + plan.rows.chunk - 1) / plan.rows.chunk);
         plan.row_jobs *= plan.rows.chunks;
         if (plan.rows.chunks > 1) plan.row_parts = plan.row_jobs * plan.beside * plan.slots;
     }
     if (plan.row_parts) plan.row_infos = row_jobs;
     if (ragged) {
-        plan.tile_slots = tokens * group / kTileRows + n_seqs;
+        plan.tile_jobs = (tokens * group / kTileRows + n_seqs) * kv_heads;
         // A tile's rows see from the first's window to the last's own token.
-        plan.tiles = split_tiles(plan.tile_slots * kv_heads,
-                                 std::min(max_length, longest + (kTileRows + group - 1) / group));
-        plan.tile_parts = plan.tiles.chunks < 2 ? 0 : tokens * heads * plan.tiles.chunks;
+        longest = std::min(max_length, longest + (kTileRows + group - 1) / group);
+        if (plan.tile_jobs < kTileRoom && longest > kLeastStages * kTileTokens) {
+            plan.tiles = TileJobs{1, kTileRoom};
+            plan.tile_jobs += kTileRoom;
+            plan.tile_parts = plan.tile_jobs * kTileRows;
+            plan.tile_infos = 2 * int64_t(n_seqs);
+        }
     }
     return plan;
 }
 
 size_t bytes_of(const Plan& plan, int width) {
     return static_cast<size_t>(plan.row_parts + plan.tile_parts) * (width + 2) * sizeof(float) +
-           static_cast<size_t>(plan.row_infos) * sizeof(int2);
+           static_cast<size_t>(plan.row_infos + plan.tile_infos) * sizeof(int2);
 }
 
 template <typename Q, bool kEight, int kJ>
@@ -1220,8 +1308,8 @@ unsigned checked_grid(int64_t groups, int threads) {
 template <typename Q>
 void launch_attend(const Attend& a, const Plan& plan, hipStream_t stream) {
     const bool eight = a.layer.type == KVSNAP_E4M3;
-    if (plan.tile_slots) {
-        const unsigned grid = checked_grid(plan.tile_slots * a.tiles.chunks * a.layer.kv_heads, kTileWaves * 64);
+    if (plan.tile_jobs) {
+        const unsigned grid = checked_grid(plan.tile_jobs, kTileWaves * 64);
         if (eight) launch_tiles<Q, true>(a, grid, stream);
         else launch_tiles<Q, false>(a, grid, stream);
         check_launched("attend's tiles");
@@ -1307,7 +1395,10 @@ int kvsnap_attend(const kvsnap_paged_layer* layer, const kvsnap_sequences* seque
         const int64_t parts = plan.row_parts + plan.tile_parts;
         a.row_parts = Parts{room, room + parts * layer->width};
         a.tile_parts = Parts{room + plan.row_parts * layer->width, a.row_parts.totals + plan.row_parts * 2};
-        if (plan.row_infos) a.row_info = reinterpret_cast<int2*>(room + parts * (layer->width + 2));
+        int2* const infos = reinterpret_cast<int2*>(room + parts * (layer->width + 2));
+        if (plan.row_infos) a.row_info = infos;
+        if (plan.tile_infos) a.tile_info = infos + plan.row_infos;
+        a.tile_jobs = static_cast<int>(plan.tile_jobs);
         require(workspace_bytes >= bytes_of(plan, layer->width), "attend: the workspace is too small");
         require(parts == 0 || (workspace && reinterpret_cast<uintptr_t>(workspace) % 16 == 0),
                 "attend: the workspace must be 16-byte aligned device memory");

@@ -413,3 +413,35 @@ def test_a_length_that_no_table_names_sees_what_its_window_names(rows):
         out = layer.attend(query.cuda(), named.cuda(), lengths, query_starts=starts)
         # as the last rows of a sequence of all 160 named tokens and 1000 more, which no table names
         check(out, query, exact, named, torch.tensor([1160], dtype=torch.int32), starts.cpu())
+
+
+@pytest.mark.parametrize("held", ["16-bit", "e4m3"])
+@pytest.mark.parametrize("count,window", [(3, None), (90, None), (300, None), (90, 700)])
+def test_chunks_over_long_contexts_are_cut_by_their_lengths(count, window, held):
+    """Tiles of rows in parts of equal length: few sequences and many (300, where a wave goes over five times 64), some
+    of one row or none, contexts from none to 2800 tokens."""
+    rng = random.Random(count)
+    added = [rng.choice([0, 1, 1, 2, 3]) for _ in range(count)]
+    lengths = [max(n, rng.choice([5, 40, 90])) for n in added]
+    for s, n, length in ((0, 70, 2800), (count // 2, 2, 1500), (count - 1, 40, 900)):
+        added[s], lengths[s] = n, length
+    blocks = sum(-(-n // 16) for n in lengths) + 1
+    layer, exact = make("vllm", blocks, 16, 1, 64, E4M3 if held == "e4m3" else FP16, count)
+    tables = tables_for(lengths, 16, blocks, count)
+    lengths = torch.tensor(lengths, dtype=torch.int32)
+    starts = torch.tensor([sum(added[:s]) for s in range(count + 1)], dtype=torch.int32)
+    query = made((sum(added), 3, 64), FP16, 7)
+    out, lse = layer.attend(query.cuda(), tables.cuda(), lengths.cuda(), query_starts=starts.cuda(), window=window,
+                            return_lse=True)
+    check(out, query, exact, tables, lengths, starts, lse=lse, window=window)
+
+
+def test_wrong_row_starts_over_long_contexts_stay_inside_the_tensors():
+    """As above, where tiles are cut: a sequence that no workgroup takes is not joined."""
+    layer, _ = make("vllm", 200, 16, 1, 64, BF16, 5)
+    tables = tables_for([1500, 900, 700], 16, 200, 5)
+    lengths = torch.tensor([1500, 900, 700], dtype=torch.int32)
+    query = made((300, 2, 64), BF16, 6).cuda()
+    for starts in ([0, 300, 0, 300], [0, 1 << 30, 0, 1 << 30], [299, 0, 300, 1], [-9, 200, 100, 300]):
+        layer.attend(query, tables.cuda(), lengths.cuda(), query_starts=torch.tensor(starts, dtype=torch.int32).cuda())
+    torch.cuda.synchronize()

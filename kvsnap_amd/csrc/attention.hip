@@ -1218,9 +1218,11 @@ constexpr int kWholeTurns = 5, kLeastTurns = 2;
 
 // Tiles whose jobs are fewer than the chip holds at once (two workgroups a CU) are cut into no more than it holds, where
 // that comes out: 12 sequences of up to 7700 tokens with 693 rows (16 heads over 8 of 128, e4m3) take 75 us; parts of one
-// length by the longest sequence's, as for three rounds, took 87, the last round being nearly empty.
-constexpr int kTileRoom = 512;
-static_assert(kTileRoom <= kTileSeqs, "tiles that are cut are of fewer sequences than a wave goes over");
+// length by the longest sequence's, as for three rounds, took 87, the last round being nearly empty.  So are up to four
+// times as many where a sequence's rows fill less than a tile, so that its tokens alone make its work: 64 sequences of up
+// to 8k tokens with 1 to 3 rows each (32 heads over 8) take 124 us, 318 whole.  A prompt's tiles are better whole, the
+// later ones first (2048 tokens: 76 us, 97 cut).
+constexpr int kTileRoom = 512, kMostCut = 4 * kTileRoom;
 
 Plan plan_of(int64_t tokens, int n_seqs, bool ragged, int heads, int kv_heads, bool eight, int64_t max_length,
              int64_t window) {
@@ -1251,10 +1253,12 @@ Plan plan_of(int64_t tokens, int n_seqs, bool ragged, int heads, int kv_heads, b
     }
     if (plan.row_parts) plan.row_infos = row_jobs;
     if (ragged) {
-        plan.tile_jobs = (tokens * group / kTileRows + n_seqs) * kv_heads;
+        const int64_t full_tiles = tokens * group / kTileRows;
+        plan.tile_jobs = (full_tiles + n_seqs) * kv_heads;
         // A tile's rows see from the first's window to the last's own token.
         longest = std::min(max_length, longest + (kTileRows + group - 1) / group);
-        if (plan.tile_jobs < kTileRoom && longest > kLeastStages * kTileTokens) {
+        if (plan.tile_jobs < (full_tiles < n_seqs ? kMostCut : kTileRoom) && n_seqs <= kTileSeqs &&
+            longest > kLeastStages * kTileTokens) {
             plan.tiles = TileJobs{1, kTileRoom};
             plan.tile_jobs += kTileRoom;
             plan.tile_parts = plan.tile_jobs * kTileRows;

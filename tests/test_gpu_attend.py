@@ -445,3 +445,20 @@ def test_wrong_row_starts_over_long_contexts_stay_inside_the_tensors():
     for starts in ([0, 300, 0, 300], [0, 1 << 30, 0, 1 << 30], [299, 0, 300, 1], [-9, 200, 100, 300]):
         layer.attend(query, tables.cuda(), lengths.cuda(), query_starts=torch.tensor(starts, dtype=torch.int32).cuda())
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("held", ["16-bit", "e4m3"])
+def test_few_rows_of_many_sequences_are_cut_by_their_lengths(held):
+    """Two to five rows of each of 80 sequences, 8 key heads: more tiles than the chip holds workgroups, none full."""
+    rng = random.Random(1)
+    added = [rng.randrange(2, 6) for _ in range(80)]
+    lengths = [rng.choice([5, 30, 70, 200]) for _ in added]
+    lengths[3], lengths[40] = 2000, 1300
+    blocks = sum(-(-n // 16) for n in lengths) + 1
+    layer, exact = make("kv_split", blocks, 16, 8, 32, E4M3 if held == "e4m3" else BF16, 2)
+    tables = tables_for(lengths, 16, blocks, 2)
+    lengths = torch.tensor(lengths, dtype=torch.int32)
+    starts = torch.tensor([sum(added[:s]) for s in range(81)], dtype=torch.int32)
+    query = made((sum(added), 8, 32), BF16, 7)
+    out, lse = layer.attend(query.cuda(), tables.cuda(), lengths.cuda(), query_starts=starts.cuda(), return_lse=True)
+    check(out, query, exact, tables, lengths, starts, lse=lse)

@@ -162,6 +162,7 @@ struct Attend {
     int2* row_info;               // [sequence, heads' group]: the first job and the parts of rows alone
     int2* tile_info;              // [sequence, 2]: the first job of its tiles and their parts, tokens of a part and tiles
     int tile_jobs;                // that there is room for
+    int least_rows;               // of a sequence whose rows are taken in tiles
     int head_tiles;            // of 16 heads, of a key head's
     int beside;                // key heads that a workgroup's waves take side by side
     int slots;                 // heads of a tile, at most
@@ -654,7 +655,7 @@ __device__ __forceinline__ TileJob even_tile_job(const Attend& a, uint32_t job) 
         stages[i] = tiles[i] = 0;
         if (s >= a.q.n_seqs) continue;
         const Rows rows = rows_of(a.q, s, a.tokens);
-        if (rows.count < 2) continue;
+        if (rows.count < a.least_rows) continue;
         tiles[i] = (rows.count * a.group + kTileRows - 1) / kTileRows;
         const Sight sight = tile_sight(a, s, rows, (tiles[i] - 1) * kTileRows);
         stages[i] = min(max((sight.high - (sight.low & ~(kTileTokens - 1)) + kTileTokens - 1) / kTileTokens, 1), 1 << 23);
@@ -717,7 +718,7 @@ __global__ __launch_bounds__(kTileWaves * 64, kD <= 128 ? 2 : 1) void attend_til
     const int sequence = same(job.sequence), kv_head = same(job.kv_head), part = same(job.part);
     const Rows rows = rows_of(a.q, sequence, a.tokens);
     const int pairs = rows.count * a.group;
-    if (rows.count < 2 || job.pair < 0 || job.pair >= pairs) return;    // no rows, or a row alone
+    if (rows.count < a.least_rows || job.pair < 0 || job.pair >= pairs) return;     // no rows, or a row alone
     const int pair0 = same(static_cast<int>(job.pair));
     const Split split{same(job.split.chunk), same(job.split.chunks)};
     const Sight sight = tile_sight(a, sequence, rows, pair0);
@@ -1179,7 +1180,7 @@ __global__ __launch_bounds__(kJoinTileThreads) void join_tiles_kernel(Attend a) 
     const int sequence = find_sequence(a.q.n_seqs, row, [&](int s) { return int64_t(a.q.query_starts[s]); });
     const Rows rows = rows_of(a.q, sequence, a.tokens);
     const int mine = row - rows.first;
-    if (mine < 0 || mine >= rows.count || rows.count == 1) return;
+    if (mine < 0 || mine >= rows.count || rows.count < a.least_rows) return;
     const int kv_head = a.group_size.divide(head), pair = mine * a.group + (head - kv_head * a.group);
     const int tile = pair / kTileRows;
     const int2 info = a.tile_info[2 * sequence], about = a.tile_info[2 * sequence + 1];
@@ -1198,7 +1199,7 @@ __global__ __launch_bounds__(kJoinTileThreads) void join_tiles_kernel(Attend a) 
 struct Plan {
     RowJobs rows;
     TileJobs tiles;
-    int beside, slots;
+    int beside, slots, least_rows = 2;
     // Parts: of all heads, 0 where rows are whole.
     int64_t row_infos = 0, tile_infos = 0, row_jobs, tile_jobs, row_parts, tile_parts;
 };
@@ -1252,6 +1253,12 @@ Plan plan_of(int64_t tokens, int n_seqs, bool ragged, int heads, int kv_heads, b
         if (plan.rows.chunks > 1) plan.row_parts = plan.row_jobs * plan.beside * plan.slots;
     }
     if (plan.row_parts) plan.row_infos = row_jobs;
+    if (ragged && n_seqs == 1 && tokens > 1) {
+        // A prompt or chunk alone: tiles take it, also where all its rows but one are padding, and there is no launch
+        // that looks for rows alone (10 us with its join).
+        plan.row_jobs = plan.row_parts = plan.row_infos = 0;
+        plan.least_rows = 1;
+    }
     if (ragged) {
         const int64_t full_tiles = tokens * group / kTileRows;
         plan.tile_jobs = (full_tiles + n_seqs) * kv_heads;
@@ -1318,20 +1325,22 @@ void launch_attend(const Attend& a, const Plan& plan, hipStream_t stream) {
         else launch_tiles<Q, false>(a, grid, stream);
         check_launched("attend's tiles");
     }
-    const unsigned grid = checked_grid(plan.row_jobs, kWaves * 64);
-    const unsigned lds = 4u * (kWaves * std::min(kHeadTile, a.group) * a.layer.width + 2 * kWaves * kHeadTile);
-    if (eight) launch_rows<Q, true>(a, grid, lds, stream);
-    else launch_rows<Q, false>(a, grid, lds, stream);
-    check_launched("attend");
+    if (plan.row_jobs) {
+        const unsigned grid = checked_grid(plan.row_jobs, kWaves * 64);
+        const unsigned lds = 4u * (kWaves * std::min(kHeadTile, a.group) * a.layer.width + 2 * kWaves * kHeadTile);
+        if (eight) launch_rows<Q, true>(a, grid, lds, stream);
+        else launch_rows<Q, false>(a, grid, lds, stream);
+        check_launched("attend's rows");
+    }
     if (plan.row_parts) {
         hipLaunchKernelGGL(join_rows_kernel<Q>, dim3(checked_grid(int64_t(a.q.n_seqs) * a.heads, kJoinThreads)),
                            dim3(kJoinThreads), 0, stream, a);
-        check_launched("attend's join");
+        check_launched("attend's joins");
     }
     if (plan.tile_parts) {
         hipLaunchKernelGGL(join_tiles_kernel<Q>, dim3(checked_grid(int64_t(a.tokens) * a.heads, kJoinTileThreads)),
                            dim3(kJoinTileThreads), 0, stream, a);
-        check_launched("attend's join");
+        check_launched("attend's joins");
     }
 }
 
@@ -1385,7 +1394,7 @@ int kvsnap_attend(const kvsnap_paged_layer* layer, const kvsnap_sequences* seque
         const Plan plan = plan_of(tokens, sequences->n_seqs, sequences->query_starts != nullptr, heads,
                                   layer->kv_heads, layer->type == KVSNAP_E4M3, std::min(max_length, named), a.window);
         a.head_tiles = (a.group + kHeadTile - 1) / kHeadTile;
-        a.beside = plan.beside, a.slots = plan.slots;
+        a.beside = plan.beside, a.slots = plan.slots, a.least_rows = plan.least_rows;
         a.block_size = Divider::of(layer->block_size);
         a.group_size = Divider::of(a.group);
         a.all_heads = Divider::of(heads);

@@ -292,7 +292,8 @@ def test_the_workspace_grows_with_what_is_split_and_is_none_for_short_rows():
     one = c_layer(kv_heads=1, width=128, token_stride=128, head_stride=128, block_stride=2048)
     size = kernel_library().kvsnap_attend_workspace_bytes
     assert size(C.addressof(one), 1, 1, 0, 4, 75, 0) == 0 and size(C.addressof(one), 0, 1, 0, 4, 1 << 20, 0) == 0
-    # a prompt's tiles are whole: what is left is one row's room for a sequence that may turn out to be one
+    # a prompt's tiles are whole; beside another sequence there is room for the parts of a row alone
+    assert size(C.addressof(held), 8192, 1, 1, 32, 8192, 0) == 0 < size(C.addressof(held), 8192, 2, 1, 32, 8192, 0)
     assert size(C.addressof(held), 8192, 1, 1, 32, 8192, 0) <= 32 << 20
     assert 0 < size(C.addressof(held), 1, 1, 0, 32, 32768, 0) <= 32 << 20
     assert size(C.addressof(held), 1, 1, 0, 32, 32768, 100) == 0

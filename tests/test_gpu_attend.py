@@ -462,3 +462,20 @@ def test_few_rows_of_many_sequences_are_cut_by_their_lengths(held):
     query = made((sum(added), 8, 32), BF16, 7)
     out, lse = layer.attend(query.cuda(), tables.cuda(), lengths.cuda(), query_starts=starts.cuda(), return_lse=True)
     check(out, query, exact, tables, lengths, starts, lse=lse)
+
+
+@pytest.mark.parametrize("length", [40, 1000])
+@pytest.mark.parametrize("added", [0, 1, 3])
+def test_one_sequence_of_few_rows_among_padding(added, length):
+    """A step of four rows for one sequence that adds fewer, one among them: the rest are padding, and stay."""
+    layer, exact = make("vllm", 70, 16, 2, 64, BF16, 8)
+    tables = tables_for([length], 16, 70, 8)
+    lengths = torch.tensor([length], dtype=torch.int32)
+    starts = torch.tensor([0, added], dtype=torch.int32)
+    query = made((4, 4, 64), BF16, 9)
+    out = torch.full((4, 4, 64), 7.0, dtype=BF16, device="cuda")
+    _, lse = layer.attend(query.cuda(), tables.cuda(), lengths.cuda(), query_starts=starts.cuda(), out=out,
+                          return_lse=True)
+    assert (out[added:] == 7).all()
+    if added:
+        check(out, query, exact, tables, lengths, starts, lse=lse, rows=slice(0, added))

@@ -246,7 +246,8 @@ __device__ __forceinline__ Cut even_cut(int n_seqs, int64_t job, const int (&uni
 #pragma unroll 1
     for (int eighths = 8; eighths <= most_eighths; ++eighths) {
         const int64_t share = (all * each * eighths + 8 * room - 1) / (8 * room);
-        chunk = (static_cast<int>(max(int64_t(least), share)) + step - 1) / step * step;
+        // (2^24 units are more than a sequence has, and their tokens still fit 32 bits)
+        chunk = (static_cast<int>(min(max(int64_t(least), share), int64_t(1) << 24)) + step - 1) / step * step;
         if (eighths == most_eighths) break;
         int jobs = 0;
 #pragma unroll

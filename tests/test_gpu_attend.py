@@ -479,3 +479,45 @@ def test_one_sequence_of_few_rows_among_padding(added, length):
     assert (out[added:] == 7).all()
     if added:
         check(out, query, exact, tables, lengths, starts, lse=lse, rows=slice(0, added))
+
+
+@pytest.mark.parametrize("captured", [False, True])
+def test_calls_at_once_on_two_streams_do_not_meet(captured):
+    """Split rows and cut tiles on two streams at a time, eager or as two captured graphs: each call has a workspace of
+    its own."""
+    layer, exact = make("kv_split", 300, 16, 2, 64, BF16, 11)
+    steps = []
+    for seed, added, lengths in ((1, [1, 40, 1], [3000, 900, 17]), (2, [70, 1], [1400, 2500])):
+        tables = tables_for(lengths, 16, 300, seed)
+        lengths = torch.tensor(lengths, dtype=torch.int32)
+        starts = torch.tensor([sum(added[:s]) for s in range(len(added) + 1)], dtype=torch.int32)
+        query = made((sum(added), 8, 64), BF16, seed)
+        steps.append((query, tables, lengths, starts))
+    on_gpu = [[t.cuda() for t in step] for step in steps]
+    call = lambda q, tables, lengths, starts: layer.attend(q, tables, lengths, query_starts=starts)
+    alone = [call(*step) for step in on_gpu]
+    streams = [torch.cuda.Stream() for _ in steps]
+    torch.cuda.synchronize()
+    if captured:
+        graphs, outs = [torch.cuda.CUDAGraph() for _ in steps], []
+        for graph, step in zip(graphs, on_gpu):
+            with torch.cuda.graph(graph):
+                outs.append(call(*step))
+    for _ in range(5):
+        if captured:
+            for out in outs:
+                out.zero_()
+            torch.cuda.synchronize()
+        else:
+            outs = [None, None]
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                if captured:
+                    graphs[i].replay()
+                else:
+                    outs[i] = call(*on_gpu[i])
+        torch.cuda.synchronize()
+        for out, want in zip(outs, alone):
+            assert torch.equal(out, want)
+    for out, (query, tables, lengths, starts) in zip(outs, steps):
+        check(out, query, exact, tables, lengths, starts)

@@ -1,0 +1,50 @@
+"""PagedCache at the ends of what its callers may ask: far blocks, far scores, small weights, odd ways of cutting."""
+import math
+import random
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from kvsnap_amd.attention import PagedCache, block_scales
+from paged_reference import E4M3, attend64, dequantised
+from test_gpu_attend import check, made
+
+pytestmark = [pytest.mark.gpu, pytest.mark.usefixtures("hip_library")]
+
+BF16, FP16 = torch.bfloat16, torch.float16
+
+
+@pytest.mark.parametrize("held,size", [("16-bit", 16), ("e4m3", 64), ("16-bit", 24)])
+def test_blocks_past_32_gib(held, size):
+    """A cache whose last blocks lie 32 GiB from its first: appends to them and attention over them, rows alone and
+    chunks long enough that whole stages of 64 tokens are seen by every row."""
+    width, dtype = 64, E4M3 if held == "e4m3" else BF16
+    block_bytes = size * 2 * width * dtype.itemsize
+    near, last = 2 ** 35 // block_bytes, 20
+    blocks = near + 1 + last                        # all of the last 20 start at or past 32 GiB
+    cache = torch.empty((blocks, 1, size, 2 * width), dtype=dtype, device="cuda")
+    assert (blocks - last) * block_bytes >= 2 ** 35
+    some = made((last, 1, size, 2 * width), torch.float32, 1).to(dtype)
+    cache[-last:].view(torch.uint8).copy_(some.view(torch.uint8))
+    scales = some_scales = None
+    if held == "e4m3":
+        scales = torch.full((blocks, 1, 2), 127, dtype=torch.uint8, device="cuda")
+        some_scales = torch.randint(124, 129, (last, 1, 2), generator=torch.Generator().manual_seed(2)).to(torch.uint8)
+        scales[-last:] = some_scales.cuda()
+    layer = PagedCache(cache, size, scales=scales)
+    exact = dequantised(some, some_scales)
+    length = last * size - 5
+    ids = random.Random(3).sample(range(last), last)
+    tables, lengths = torch.tensor([ids], dtype=torch.int32), torch.tensor([length], dtype=torch.int32)
+    far = (tables + (blocks - last)).cuda()
+    for rows in (1, 70):
+        query = made((rows, 2, width), BF16, 4)
+        starts = torch.tensor([0, rows], dtype=torch.int32)
+        out = layer.attend(query.cuda(), far, lengths.cuda(), query_starts=starts.cuda())
+        check(out, query, exact, tables, lengths, starts)
+    if held == "16-bit":
+        key, value = made((1, 1, width), BF16, 5), made((1, 1, width), BF16, 6)
+        layer.append(key.cuda(), value.cuda(), far, lengths.cuda())
+        some[ids[-1], 0, (length - 1) % size] = torch.cat([key[0, 0], value[0, 0]])
+        assert torch.equal(cache[-last:].cpu(), some)

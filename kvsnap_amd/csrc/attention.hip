@@ -116,6 +116,15 @@ __device__ __forceinline__ float sum_across_halves(float x) {
     return bits<float>(halves[0]) + bits<float>(halves[1]);
 }
 
+// Weights are 2^(score * factor - top * factor), rounded once behind the second product.  What rounding that product
+// moves is common to a row's weights and falls out, while it is little: whether some row's is more than 2^-14 (largest
+// scores from some 2^10 binary logarithms on).  There scores are taken less `top` before they meet the factor: exact
+// for the tokens that count, and never a power that overflows or leaves every weight 0.
+__device__ __forceinline__ bool rounds_far(float top, float factor) {
+    return __ballot(!(__builtin_fabsf(__builtin_fmaf(top, factor, -(top * factor))) <= 0x1p-14f) &&
+                    top != -__builtin_inff()) != 0;
+}
+
 // One over a row's sum: 0 for a row that sees nothing, and NaN stays.
 __device__ __forceinline__ float over(float total) { return total > 0 ? 1.0f / total : total == 0 ? 0.0f : total; }
 
@@ -367,6 +376,7 @@ __global__ __launch_bounds__(kWaves * 64, kEight && kJ <= 8 ? 4 : 2) void attend
     for (int j = 0; j < kJ; ++j) sum[j] = f32x4{0, 0, 0, 0};
     float top = -__builtin_inff(), total = 0;
     const float factor = a.scale * kLog2e;
+    bool far = false;
 
     const int base = (sight.low & ~(kTile - 1)) + part * job.chunk * kTile;
     const int stop = part == parts - 1 ? sight.high : min(sight.high, base + job.chunk * kTile);
@@ -518,8 +528,14 @@ __global__ __launch_bounds__(kWaves * 64, kEight && kJ <= 8 ? 4 : 2) void attend
 #pragma unroll
             for (int j = 0; j < kJ; ++j) sum[j] *= shrink;
             top = grown;
+            far = rounds_far(top, factor);
         }
-        const float against = top == -__builtin_inff() ? 0.0f : top * factor;
+        float against = top == -__builtin_inff() ? 0.0f : top * factor;
+        if (far) {
+#pragma unroll
+            for (int t = 0; t < 8; ++t) score[t >> 2][t & 3] -= top == -__builtin_inff() ? 0.0f : top;
+            against = 0;
+        }
         Vec p[kTerms];
 #pragma unroll
         for (int t = 0; t < 8; ++t) {
@@ -897,7 +913,8 @@ __global__ __launch_bounds__(kTileWaves * 64, kD <= 128 ? 2 : 1) void attend_til
 #pragma unroll
         for (int i = 0; i < 16; ++i) sum[b][i] = 0;
     float top = -__builtin_inff(), total = 0;
-    const float factor = a.scale * kLog2e, slack = __builtin_fminf(8.0f / factor, 1e30f);   // finite: -inf + slack is -inf
+    const float factor = a.scale * kLog2e, slack = __builtin_fminf(8.0f / factor, 1e30f);
+    bool far = false;
 
     if (thread < 6) odd[thread >> 1][thread & 1] = 0;
     int block = named_block(base);
@@ -948,7 +965,7 @@ __global__ __launch_bounds__(kTileWaves * 64, kD <= 128 ? 2 : 1) void attend_til
         most = max_across_halves(most);
         // Weights are relative to a score at most 2^8 below the largest: they keep their relative precision, and the
         // sums are scaled again in few tiles.
-        if (__ballot(most > top + slack)) {
+        if (__ballot(most - top > slack)) {
             const float grown = __builtin_fmaxf(top, most);
             const float shrink = top == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((top - grown) * factor);
             total *= shrink;
@@ -957,8 +974,16 @@ __global__ __launch_bounds__(kTileWaves * 64, kD <= 128 ? 2 : 1) void attend_til
 #pragma unroll
                 for (int i = 0; i < 16; ++i) sum[b][i] *= shrink;
             top = grown;
+            far = rounds_far(top, factor);
         }
-        const float against = top == -__builtin_inff() ? 0.0f : top * factor;
+        float against = top == -__builtin_inff() ? 0.0f : top * factor;
+        if (far) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) score[h][i] -= top == -__builtin_inff() ? 0.0f : top;
+            against = 0;
+        }
         Vec p[4][kTerms];
 #pragma unroll
         for (int h = 0; h < 2; ++h)

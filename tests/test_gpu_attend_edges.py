@@ -48,3 +48,32 @@ def test_blocks_past_32_gib(held, size):
         layer.append(key.cuda(), value.cuda(), far, lengths.cuda())
         some[ids[-1], 0, (length - 1) % size] = torch.cat([key[0, 0], value[0, 0]])
         assert torch.equal(cache[-last:].cpu(), some)
+
+
+@pytest.mark.parametrize("rows", [1, 50])
+@pytest.mark.parametrize("held", ["16-bit", "e4m3"])
+@pytest.mark.parametrize("dtype,power", [(FP16, 15), (BF16, 15), (BF16, 45)])
+def test_scores_far_beyond_the_exponentials_range(dtype, power, held, rows):
+    """Queries and keys of 2^power: scores of 2^33 and more, all alike but for every third token's, which are less by
+    far more than any exponent.  Every product and sum is exact, so weights are 0 or alike, and the check's bound
+    holds as it is."""
+    size, kv, width, length = 16, 1, 64, 1500
+    blocks = -(-length // size)
+    shape = (2, blocks, size, kv, width)
+    cache, scales = made(shape, torch.float32, 1), None
+    cache[0] = 1.0
+    cache[0, :, ::3] = 0.875
+    if held == "e4m3":
+        cache, scales = cache.to(E4M3), torch.full((blocks, kv, 2), 127, dtype=torch.uint8)
+        scales[..., 0] += power
+    else:
+        cache[0] *= 2.0 ** power
+        cache = cache.to(dtype)
+    exact = dequantised(cache, scales)
+    layer = PagedCache(cache.cuda(), size, scales=None if scales is None else scales.cuda())
+    tables, lengths = torch.randperm(blocks, dtype=torch.int32)[None], torch.tensor([length], dtype=torch.int32)
+    starts = torch.tensor([0, rows], dtype=torch.int32)
+    query = torch.full((rows, 2, width), 2.0 ** power, dtype=dtype)
+    query[:, 1] = -query[:, 1]
+    out, lse = layer.attend(query.cuda(), tables.cuda(), lengths.cuda(), query_starts=starts.cuda(), return_lse=True)
+    check(out, query, exact, tables, lengths, starts, lse=lse)

@@ -119,7 +119,9 @@ size_t kvsnap_attend_workspace_bytes(const kvsnap_paged_layer* layer, int64_t to
  * zeros and a log sum of -inf.
  * Softmax, sums and products' sums are fp32; weights are rounded to 16 bits
  * before they meet the values (to two such terms for fp16 queries over an
- * e4m3 cache), and an e4m3 cache's values are exact in bf16.  lse, or NULL:
+ * e4m3 cache; an fp16 cache's by at least 2^-30 of the largest weight among
+ * 64 tokens, which moves an output by at most 2^-24 of the largest value),
+ * and an e4m3 cache's values are exact in bf16.  lse, or NULL:
  * fp32 [tokens, heads], the natural logarithm of each row's sum of
  * exponentials.  max_length, at least every sequence's length if it can be
  * known, only shapes the launch.  workspace: 16-byte aligned scratch of

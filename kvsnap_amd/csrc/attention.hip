@@ -65,6 +65,38 @@ struct Shape<__bf16, true> {
     static constexpr int kTerms = 1;
 };
 
+// What weights are relative to: a score near the largest so far, `slack` binary logarithms below it at most.
+//
+// Weights of an fp16 cache's values are fp16 too, whose range is short: below 2^-14 they lose bits, at 2^-25 they are
+// gone from the product while they count in the sum.  So they are 2^kLift times as large, fp16's range from its top
+// down, and their reference follows the tiles' largest scores down as well as up: where one is more than kFall under it,
+// it moves to just below that.  A weight is then rounded by half a step, or by 2^-25 where its tile's largest is at least
+// 2^(kLift - kFall): whatever the length, that moves a row's out by at most the tile's tokens (64, or 32 for rows alone)
+// times 2^-30 of the largest value.
+template <typename T>
+struct Weights {
+    static constexpr bool kFollow = std::is_same_v<T, _Float16>;
+    static constexpr float kLift = kFollow ? 9 : 0, kDrop = kFollow ? 0x1p-9f : 1;      // kDrop: 2^-kLift
+    static constexpr float kFall = 4;
+    float factor, slack, fall;
+
+    __device__ __forceinline__ Weights(float factor, float slack_of)
+        : factor(factor), slack(__builtin_fminf(slack_of / factor, 1e30f)), fall(__builtin_fminf(kFall / factor, 1e30f)) {}
+
+    // Whether a row's reference moves for scores of at most `most`, and where to.  Down no farther than sums of `total`,
+    // the row's, have room to grow: to 2^90, and values are at most 2^16.
+    __device__ __forceinline__ bool moves(float top, float most) const {
+        return most - top > slack || (kFollow && most - top < -fall);
+    }
+    __device__ __forceinline__ float moved(float top, float most, float total) const {
+        if (!kFollow) return __builtin_fmaxf(top, most);
+        if (most == -__builtin_inff() || !moves(top, most)) return top;
+        const float below = most - __builtin_fminf(1.0f / factor, 1e30f);
+        if (!(below < top)) return below;
+        return __builtin_fmaxf(below, top - __builtin_fmaxf(90.0f - __builtin_log2f(total), 0.0f) / factor);
+    }
+};
+
 __device__ __forceinline__ void two_terms(float x, bf16x8& first, bf16x8& rest, int i) {
     first[i] = static_cast<__bf16>(x);
     rest[i] = static_cast<__bf16>(x - static_cast<float>(first[i]));
@@ -328,6 +360,7 @@ template <typename Q, bool kEight, int kJ, bool kWhole, bool kExact>
 __global__ __launch_bounds__(kWaves * 64, kEight && kJ <= 8 ? 4 : 2) void attend_row_kernel(Attend a) {
     using T = typename Shape<Q, kEight>::T;
     using Vec = typename Matrix<T>::Vec;
+    using W = Weights<T>;
     constexpr int kTerms = Shape<Q, kEight>::kTerms;
     constexpr int kSteps = kJ / 2;                          // products of 32 values along a row
     using Loads = Tile<kEight, kJ>;
@@ -376,6 +409,7 @@ __global__ __launch_bounds__(kWaves * 64, kEight && kJ <= 8 ? 4 : 2) void attend
     for (int j = 0; j < kJ; ++j) sum[j] = f32x4{0, 0, 0, 0};
     float top = -__builtin_inff(), total = 0;
     const float factor = a.scale * kLog2e;
+    const W weights(factor, W::kFollow ? 6 : 0);
     bool far = false;
 
     const int base = (sight.low & ~(kTile - 1)) + part * job.chunk * kTile;
@@ -521,20 +555,20 @@ __global__ __launch_bounds__(kWaves * 64, kEight && kJ <= 8 ? 4 : 2) void attend
 #pragma unroll
         for (int t = 0; t < 8; ++t) most = __builtin_fmaxf(most, score[t >> 2][t & 3]);
         most = max_across_groups(most);
-        if (__ballot(most > top)) {
-            const float grown = __builtin_fmaxf(top, most);
-            const float shrink = top == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((top - grown) * factor);
+        if (__ballot(weights.moves(top, most))) {
+            const float to = weights.moved(top, most, W::kFollow ? sum_across_groups(total) : 0);
+            const float shrink = top == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((top - to) * factor);
             total *= shrink;
 #pragma unroll
             for (int j = 0; j < kJ; ++j) sum[j] *= shrink;
-            top = grown;
+            top = to;
             far = rounds_far(top, factor);
         }
-        float against = top == -__builtin_inff() ? 0.0f : top * factor;
+        float against = top == -__builtin_inff() ? 0.0f : __builtin_fmaf(top, factor, -W::kLift);
         if (far) {
 #pragma unroll
             for (int t = 0; t < 8; ++t) score[t >> 2][t & 3] -= top == -__builtin_inff() ? 0.0f : top;
-            against = 0;
+            against = -W::kLift;
         }
         Vec p[kTerms];
 #pragma unroll
@@ -605,7 +639,8 @@ __global__ __launch_bounds__(kWaves * 64, kEight && kJ <= 8 ? 4 : 2) void attend
         float x = 0, y = 0, all = 0;
         for (int w = wave % beside; w < kWaves; w += beside) {
             const float mine = tops[w * kHeadTile + head];
-            const float share = mine == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((mine - most) * factor);
+            const float share = mine == -__builtin_inff() ? 0.0f
+                                                           : __builtin_amdgcn_exp2f((mine - most) * factor) * W::kDrop;
             const float* const from = shared + (w * heads + head) * width + d;
             x += from[0] * share;
             y += from[1] * share;
@@ -716,6 +751,7 @@ template <typename Q, bool kEight, int kD, bool kWhole>
 __global__ __launch_bounds__(kTileWaves * 64, kD <= 128 ? 2 : 1) void attend_tile_kernel(Attend a) {
     using T = typename Shape<Q, kEight>::T;
     using Vec = typename Matrix<T>::Vec;
+    using W = Weights<T>;
     constexpr int kTerms = Shape<Q, kEight>::kTerms;
     constexpr int kBytes = kEight ? 1 : 2;
     constexpr int kSteps = kD / 16, kBlocks = kD / 32;
@@ -913,7 +949,8 @@ __global__ __launch_bounds__(kTileWaves * 64, kD <= 128 ? 2 : 1) void attend_til
 #pragma unroll
         for (int i = 0; i < 16; ++i) sum[b][i] = 0;
     float top = -__builtin_inff(), total = 0;
-    const float factor = a.scale * kLog2e, slack = __builtin_fminf(8.0f / factor, 1e30f);
+    const float factor = a.scale * kLog2e;
+    const W weights(factor, W::kFollow ? 6 : 8);
     bool far = false;
 
     if (thread < 6) odd[thread >> 1][thread & 1] = 0;
@@ -963,26 +1000,26 @@ __global__ __launch_bounds__(kTileWaves * 64, kD <= 128 ? 2 : 1) void attend_til
 #pragma unroll
             for (int i = 0; i < 16; ++i) most = __builtin_fmaxf(most, score[h][i]);
         most = max_across_halves(most);
-        // Weights are relative to a score at most 2^8 below the largest: they keep their relative precision, and the
-        // sums are scaled again in few tiles.
-        if (__ballot(most - top > slack)) {
-            const float grown = __builtin_fmaxf(top, most);
-            const float shrink = top == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((top - grown) * factor);
+        // Weights may be up to 2^8 (fp16: 2^6): they keep their relative precision, and the sums are scaled again in few
+        // tiles.
+        if (__ballot(weights.moves(top, most))) {
+            const float to = weights.moved(top, most, W::kFollow ? sum_across_halves(total) : 0);
+            const float shrink = top == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((top - to) * factor);
             total *= shrink;
 #pragma unroll
             for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) sum[b][i] *= shrink;
-            top = grown;
+            top = to;
             far = rounds_far(top, factor);
         }
-        float against = top == -__builtin_inff() ? 0.0f : top * factor;
+        float against = top == -__builtin_inff() ? 0.0f : __builtin_fmaf(top, factor, -W::kLift);
         if (far) {
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) score[h][i] -= top == -__builtin_inff() ? 0.0f : top;
-            against = 0;
+            against = -W::kLift;
         }
         Vec p[4][kTerms];
 #pragma unroll
@@ -1093,7 +1130,8 @@ __global__ __launch_bounds__(kTileWaves * 64, kD <= 128 ? 2 : 1) void attend_til
     total = sum_across_halves(total);
     if (!real) return;
     const int64_t index = row * a.heads + head;
-    const float share = parts > 1 ? 1.0f : over(total);
+    const float share = parts > 1 ? W::kDrop : over(total);
+    total *= W::kDrop;
     const int64_t at_part = int64_t(blockIdx.x) * kTileRows + pair - pair0;
     float* const sums = a.tile_parts.sums + at_part * width;
     Q* const out = static_cast<Q*>(a.out) + row * a.out_token_stride + head * a.out_head_stride;
@@ -1104,8 +1142,8 @@ __global__ __launch_bounds__(kTileWaves * 64, kD <= 128 ? 2 : 1) void attend_til
             const int d = 32 * b + 8 * i + 4 * half;
             if (d >= width) continue;
             if (parts > 1) {
-                *reinterpret_cast<f32x4*>(sums + d) = f32x4{sum[b][4 * i], sum[b][4 * i + 1], sum[b][4 * i + 2],
-                                                           sum[b][4 * i + 3]};
+                *reinterpret_cast<f32x4*>(sums + d) = f32x4{sum[b][4 * i] * share, sum[b][4 * i + 1] * share,
+                                                           sum[b][4 * i + 2] * share, sum[b][4 * i + 3] * share};
             } else {
                 typedef Q Four __attribute__((ext_vector_type(4)));
                 Four four;

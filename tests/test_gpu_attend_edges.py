@@ -77,3 +77,33 @@ def test_scores_far_beyond_the_exponentials_range(dtype, power, held, rows):
     query[:, 1] = -query[:, 1]
     out, lse = layer.attend(query.cuda(), tables.cuda(), lengths.cuda(), query_starts=starts.cuda(), return_lse=True)
     check(out, query, exact, tables, lengths, starts, lse=lse)
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+@pytest.mark.parametrize("sink", ["first", "middle", "last seen by all"])
+def test_small_weights_behind_one_that_takes_all_in_fp16(sink, rows):
+    """One token's weight is 2^14 to 2^30 times any other's and its value 0, so the output is the others' alone.
+
+    The check's roundings, and fp16's least steps: a weight beside the large one, in the same 64 tokens, is rounded by
+    up to 2^-25 of 2^-5 of that one, and 64 of those, over a sum that is at least the large one, move the output by at
+    most 2^-24 of the largest value."""
+    size, kv, width, length = 16, 1, 64, 3000
+    blocks = -(-length // size)
+    at = {"first": 0, "middle": 1333, "last seen by all": length - rows}[sink]
+    tables = torch.randperm(blocks, generator=torch.Generator().manual_seed(1)).to(torch.int32)[None]
+    cache = torch.zeros((2, blocks, size, kv, width))
+    cache[1] = 0.5 + torch.rand(cache[1].shape, generator=torch.Generator().manual_seed(2))
+    block, slot = int(tables[0, at // size]), at % size
+    cache[0, block, slot], cache[1, block, slot] = 1.0, 0.0
+    cache = cache.to(FP16)
+    keys, values = (side.double() for side in cache)
+    times = torch.tensor([14.5, 22.0, 25.2, 30.0])           # in binary logarithms: 64 q / 8 = times * ln 2
+    query = (times * math.log(2) / 8)[None, :, None].expand(rows, 4, width).to(FP16).contiguous()
+    lengths, starts = torch.tensor([length], dtype=torch.int32), torch.tensor([0, rows], dtype=torch.int32)
+    got, lse = PagedCache(cache.cuda(), size).attend(query.cuda(), tables.cuda(), lengths.cuda(),
+                                                     query_starts=starts.cuda(), return_lse=True)
+    want, want_lse = attend64(query, keys, values, tables, lengths, starts)      # values are not negative: the spread too
+    bound = (2.0 ** -10 + 2.0 ** -11) * want + 2.0 ** -24 + 2.0 ** -24 * 1.5
+    off = (got.cpu().double() - want).abs() - bound
+    assert off.max() <= 0, (off.amax((0, 2)) / want.amin((0, 2))).tolist()
+    assert ((lse.cpu().double() - want_lse).abs() <= 2.0 ** -12 + 2.0 ** -22 * want_lse.abs()).all()

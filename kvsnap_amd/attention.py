@@ -15,7 +15,8 @@ them may be captured in a graph and replayed over changed tables.  Launches go t
 device.  There is no CPU fallback: without the HIP library every call raises.
 
 The kernels' contract is in ``include/kvsnap_attention.h``; arguments are checked in ``csrc/binding.cpp``.  No
-gradient is recorded: a tensor that requires one is refused outside ``torch.no_grad()``.
+gradient is recorded: a tensor that requires one is refused outside ``torch.no_grad()``, and one that carries a
+forward-mode tangent is refused.
 """
 from __future__ import annotations
 

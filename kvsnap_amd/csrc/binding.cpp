@@ -7,6 +7,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/GradMode.h>
 #include <c10/hip/HIPStream.h>
@@ -81,6 +82,14 @@ std::string shape_of(const at::Tensor& t) {
     return text.str();
 }
 
+// The calls record nothing for either direction of differentiation: what would be lost is refused.
+void check_undifferentiated(const at::Tensor& t, const char* what) {
+    if (t.requires_grad() && at::GradMode::is_enabled())
+        refuse(what, " requires a gradient, and no gradient is recorded here: call under torch.no_grad()");
+    if (c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined())
+        refuse(what, " carries a forward-mode tangent, and none is computed here");
+}
+
 // A [tokens, heads, width] tensor (a negative size: any) whose last axis is contiguous.
 void check_rows(const at::Tensor& t, const char* what, int64_t tokens, int64_t heads, int64_t width) {
     const auto differs = [&](int axis, int64_t want) { return want >= 0 && t.size(axis) != want; };
@@ -89,8 +98,7 @@ void check_rows(const at::Tensor& t, const char* what, int64_t tokens, int64_t h
         refuse(what, " must be [", size(tokens), ", ", size(heads), ", ", size(width), "], not ", shape_of(t));
     }
     if (t.stride(2) != 1 && t.size(2) > 1) refuse(what, ": the last axis must be contiguous");
-    if (t.requires_grad() && at::GradMode::is_enabled())
-        refuse(what, " requires a gradient, and no gradient is recorded here: call under torch.no_grad()");
+    check_undifferentiated(t, what);
 }
 
 void check_device(const at::Device& device, std::initializer_list<const at::Tensor*> tensors) {

@@ -124,6 +124,7 @@ Rotation rotation_of(PyObject* rotary, PyObject* positions, PyObject* axes, bool
     if (r.table->dim() != 3 || r.table->size(2) != 2 || r.table->scalar_type() != at::kFloat ||
         !r.table->is_contiguous())
         refuse("a rotary table is a contiguous float32 [positions, pairs, 2] tensor");
+    check_undifferentiated(*r.table, "a rotary table");
     const int64_t pairs = r.table->size(1);
     if (pairs == 0 || pairs % 8 || 2 * pairs > width)
         refuse("a rotary table's pairs must be a multiple of 8 and at most ", width / 2, ", not ", pairs);
@@ -293,9 +294,11 @@ struct Layer {
     const kvsnap_paged_layer* raw;
     at::Device device;
 
-    Layer(PyObject* address, PyObject* on)
+    Layer(PyObject* address, PyObject* cache)
         : raw(reinterpret_cast<const kvsnap_paged_layer*>(static_cast<uintptr_t>(whole(address)))),
-          device(THPVariable_Unpack(on).device()) {}
+          device(THPVariable_Unpack(cache).device()) {
+        check_undifferentiated(THPVariable_Unpack(cache), "the cache");
+    }
 };
 
 // append(layer, cache, key, value, block_tables, lengths, query_starts, query, positions, rotary, axes, interleaved,

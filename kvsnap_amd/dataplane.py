@@ -893,9 +893,21 @@ class TorchBlockDataPlane:
 
     def paged_cache(self, name, *, scales=None):
         """The registered cache ``name`` for the operators that fill and read it (``kvsnap_amd.attention``); an e4m3
-        one with its layer's ``scales``."""
+        one with its layer's ``scales``, a view of the rows that the plane saves with its blocks."""
         from .attention import PagedCache
-        return PagedCache(self.caches[name], self.block_size, scales=scales)
+        cache = PagedCache(self.caches[name], self.block_size, scales=scales)
+        if scales is not None:
+            rows = self.scales
+            if rows is None:
+                raise ValueError(f"KV cache {name!r}: the plane was registered without scales and would save its blocks "
+                                 "without theirs")
+            first = scales.data_ptr() - rows.data_ptr()
+            used = sum((size - 1) * stride for size, stride in zip(scales.shape[1:], scales.stride()[1:])) + 1
+            if (first < 0 or first + used > rows.shape[1] or scales.shape[0] > rows.shape[0]
+                    or scales.stride(0) != rows.stride(0)):
+                raise ValueError(f"KV cache {name!r}: the scales are no view of the plane's own: its blocks would be "
+                                 "saved and restored without them")
+        return cache
 
     def _num_blocks(self, tensor):
         return tensor.shape[1] if tensor.ndim == 5 else tensor.shape[0]

@@ -4,7 +4,7 @@ import pytest
 torch = pytest.importorskip("torch")
 import torch.autograd.forward_ad as forward_ad
 
-from kvsnap_amd.attention import PagedCache, rotate
+from kvsnap_amd.attention import PagedCache, block_scales, rotate
 from test_attention_host import ON_CPU, append, attend, built, layer, step  # noqa: F401  (built: a fixture)
 
 
@@ -43,3 +43,28 @@ def test_a_gradient_of_the_cache_or_of_the_table_is_refused_not_dropped():
             call()
         with torch.no_grad(), pytest.raises(ValueError, match=ON_CPU):
             call()
+
+
+def test_a_plane_refuses_scales_that_it_does_not_save():
+    """Its blocks would come back with the scales that some other block had."""
+    from kvsnap_amd.dataplane import TorchBlockDataPlane
+    plane = object.__new__(TorchBlockDataPlane)
+    plane.block_size = 16
+    plane.caches = {f"layer.{i}": torch.zeros((2, 4, 16, 2, 64)).to(torch.float8_e4m3fn) for i in range(3)}
+    plane.scales, views = block_scales(5, 3, 2)
+    views = [view[:4] for view in views]            # more rows than the caches have blocks
+    for name, view in zip(plane.caches, views):
+        assert plane.paged_cache(name, scales=view).scales is view
+    wide, wide_views = block_scales(4, 9, 2)
+    for other in (block_scales(4, 3, 2)[1][0], torch.zeros((4, 2, 2), dtype=torch.uint8), wide_views[8],
+                  plane.scales[0].view(torch.uint8).view(4, 2, 2),              # all of one block's row
+                  plane.scales.view(torch.uint8).flatten().as_strided((4, 2, 2), (16, 2, 1), 14)):      # into the next
+        with pytest.raises(ValueError, match="no view of the plane's own"):
+            plane.paged_cache("layer.0", scales=other)
+    plane.scales = wide
+    assert plane.paged_cache("layer.0", scales=wide_views[8]).scales is wide_views[8]
+    plane.scales = None
+    with pytest.raises(ValueError, match="registered without scales"):
+        plane.paged_cache("layer.0", scales=views[0])
+    plane.caches["plain"] = torch.zeros((2, 4, 16, 2, 64), dtype=torch.bfloat16)
+    assert plane.paged_cache("plain").scales is None

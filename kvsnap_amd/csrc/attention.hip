@@ -1415,7 +1415,7 @@ extern "C" {
 
 size_t kvsnap_attend_workspace_bytes(const kvsnap_paged_layer* layer, int64_t tokens, int n_seqs, int ragged, int heads,
                                      int64_t max_length, int64_t window) {
-    if (!layer || tokens <= 0 || n_seqs <= 0 || heads <= 0 || layer->kv_heads <= 0) return 0;
+    if (!layer || tokens <= 0 || n_seqs <= 0 || heads <= 0 || layer->kv_heads <= 0 || heads % layer->kv_heads) return 0;
     return bytes_of(plan_of(tokens, n_seqs, ragged, heads, layer->kv_heads, layer->type == KVSNAP_E4M3, max_length,
                             std::min<int64_t>(window, 1 << 30)),
                     layer->width);

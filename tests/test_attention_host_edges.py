@@ -1,4 +1,9 @@
 """What kvsnap_amd.attention refuses at its edges, without a GPU."""
+import os
+import subprocess
+import sys
+from pathlib import Path
+
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -68,3 +73,21 @@ def test_a_plane_refuses_scales_that_it_does_not_save():
         plane.paged_cache("layer.0", scales=views[0])
     plane.caches["plain"] = torch.zeros((2, 4, 16, 2, 64), dtype=torch.bfloat16)
     assert plane.paged_cache("plain").scales is None
+
+
+def test_the_workspace_of_heads_that_share_no_key_head_ends_no_process():
+    """Fewer query heads than key heads, from C: a division by zero would be the whole process's end, so in its own."""
+    program = """
+import ctypes as C
+from test_attention_host import c_layer
+from kvsnap_amd.native import kernel_library
+size = kernel_library().kvsnap_attend_workspace_bytes
+for heads in (1, 3, 7, 9, 12):
+    for ragged in (0, 1):
+        assert size(C.addressof(c_layer(kv_heads=8)), 64, 2, ragged, heads, 1 << 20, 0) == 0
+assert size(C.addressof(c_layer(kv_heads=8)), 64, 2, 1, 16, 1 << 20, 0) > 0
+"""
+    here = Path(__file__).resolve().parent
+    done = subprocess.run([sys.executable, "-c", program], cwd=here, env={**os.environ, "PYTHONPATH": f"{here}:{here.parent}"},
+                          capture_output=True, text=True)
+    assert done.returncode == 0, done.stderr

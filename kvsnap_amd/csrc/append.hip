@@ -390,7 +390,7 @@ kvsnap_rotation checked_rotation(const kvsnap_rotation* rotation, int width) {
 }
 
 uint32_t counted_items(int64_t a, int64_t b, int64_t c) {
-    const int64_t n = a * b * c;
+    const __int128 n = __int128(a) * b * c;
     require(n < (int64_t(1) << 31), "too many values for one launch");
     return static_cast<uint32_t>(n);
 }

@@ -1,4 +1,5 @@
 """What kvsnap_amd.attention refuses at its edges, without a GPU."""
+import ctypes as C
 import os
 import subprocess
 import sys
@@ -10,7 +11,14 @@ torch = pytest.importorskip("torch")
 import torch.autograd.forward_ad as forward_ad
 
 from kvsnap_amd.attention import PagedCache, block_scales, rotate
-from test_attention_host import ON_CPU, append, attend, built, layer, step  # noqa: F401  (built: a fixture)
+from kvsnap_amd.native import kernel_library
+from test_attention_host import (ON_CPU, Sequences, append, attend, built, c_layer, layer,  # noqa: F401  (a fixture)
+                                 step)
+
+
+class Rotation(C.Structure):
+    _fields_ = [("angles", C.c_void_p), ("positions", C.c_void_p), ("rows", C.c_int64), ("axis_stride", C.c_int64),
+                *((name, C.c_int32) for name in ("pairs", "interleaved", "narrow", "inverse")), ("axes", C.c_uint16 * 16)]
 
 
 @pytest.mark.parametrize("name", ["query", "key", "value", "query_out"])
@@ -91,3 +99,15 @@ assert size(C.addressof(c_layer(kv_heads=8)), 64, 2, 1, 16, 1 << 20, 0) > 0
     done = subprocess.run([sys.executable, "-c", program], cwd=here, env={**os.environ, "PYTHONPATH": f"{here}:{here.parent}"},
                           capture_output=True, text=True)
     assert done.returncode == 0, done.stderr
+
+
+def test_the_c_entry_points_refuse_counts_whose_product_passes_64_bits():
+    """2^40 + 1 rows of 2^24 heads in units of 16 values: 2^64 + 2^24 units for one launch."""
+    lib = kernel_library()
+    turns = Rotation(angles=4096, positions=4096, rows=10, pairs=8)
+    assert lib.kvsnap_rotate(4096, 16, 16, 4096, 16, 16, (1 << 40) + 1, 1 << 24, 16, 0, C.addressof(turns), 0) == -1
+    assert "too many values" in lib.kvsnap_cuda_error().decode()
+    sequences = Sequences(4096, 4096, 4096, 2, 2, 1)
+    assert lib.kvsnap_append(C.addressof(c_layer(width=16)), C.addressof(sequences), None, 4096, 16, 16, 4096, 16, 16, 4096,
+                             16, 16, 4096, 16, 16, (1 << 31) - 1, (1 << 31) - 1, 0, 0) == -1
+    assert "too many values" in lib.kvsnap_cuda_error().decode()

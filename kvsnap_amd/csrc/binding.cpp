@@ -122,8 +122,8 @@ Rotation rotation_of(PyObject* rotary, PyObject* positions, PyObject* axes, bool
     }
     r.table = &tensor(rotary, "a rotary table");
     if (r.table->dim() != 3 || r.table->size(2) != 2 || r.table->scalar_type() != at::kFloat ||
-        !r.table->is_contiguous())
-        refuse("a rotary table is a contiguous float32 [positions, pairs, 2] tensor");
+        !r.table->is_contiguous() || r.table->size(0) == 0)
+        refuse("a rotary table is a contiguous float32 [positions, pairs, 2] tensor of one position or more");
     check_undifferentiated(*r.table, "a rotary table");
     const int64_t pairs = r.table->size(1);
     if (pairs == 0 || pairs % 8 || 2 * pairs > width)

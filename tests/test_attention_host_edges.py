@@ -111,3 +111,12 @@ def test_the_c_entry_points_refuse_counts_whose_product_passes_64_bits():
     assert lib.kvsnap_append(C.addressof(c_layer(width=16)), C.addressof(sequences), None, 4096, 16, 16, 4096, 16, 16, 4096,
                              16, 16, 4096, 16, 16, (1 << 31) - 1, (1 << 31) - 1, 0, 0) == -1
     assert "too many values" in lib.kvsnap_cuda_error().decode()
+
+
+def test_a_rotary_table_of_no_positions_is_refused():
+    """Its address is none, which to the library means that nothing is turned."""
+    none = torch.zeros((0, 32, 2))
+    with pytest.raises(ValueError, match="of one position or more"):
+        append(layer(), step(), rotary=none)
+    with pytest.raises(ValueError, match="of one position or more"):
+        rotate(torch.zeros((3, 2, 64)), torch.zeros(3, dtype=torch.int64), none)

@@ -81,7 +81,8 @@ typedef struct kvsnap_rotation {
 
 /* out = x with every head turned, for x and out of `tokens` rows of `heads`
  * heads of `width` values of type (bf16, fp16 or fp32), strides in elements;
- * `inverse` turns back, which is also the gradient's turn.  out may be x.
+ * `inverse` turns back, which is also the gradient's turn.  out may be x, and
+ * otherwise overlaps no part of it.
  * width a multiple of 16 up to 256; rows, heads and angles 16-byte aligned. */
 int kvsnap_rotate(const void* x, int64_t x_token_stride, int64_t x_head_stride, void* out, int64_t out_token_stride,
                   int64_t out_head_stride, int64_t tokens, int heads, int width, int type,
@@ -90,14 +91,14 @@ int kvsnap_rotate(const void* x, int64_t x_token_stride, int64_t x_head_stride, 
 /* One step's keys and values ([tokens, kv_heads, width] of type bf16 or fp16)
  * into their sequences' blocks, the keys turned on the way, and `query`
  * ([tokens, heads, width], or NULL) turned into query_out (which may be
- * query).  A 16-bit cache is of the same type.  Into an e4m3 cache a block's
- * values go with the least power of two that keeps the new ones within e4m3's
- * 448, or the block's scale where slots filled before this step need more;
- * where the new ones do, the slots before them are rounded again to the new
- * scale.  Slots past the sequence's length are left as they are, and a value
- * that is not finite is stored as NaN.  Sequences of one call share no block
- * that it writes.  lengths[s] is at least the rows of sequence s; rows ahead
- * of position 0 are padding too. */
+ * query, and otherwise overlaps nothing that is read).  A 16-bit cache is of
+ * the same type.  Into an e4m3 cache a block's values go with the least power
+ * of two that keeps the new ones within e4m3's 448, or the block's scale where
+ * slots filled before this step need more; where the new ones do, the slots
+ * before them are rounded again to the new scale.  Slots past the sequence's
+ * length are left as they are, and a value that is not finite is stored as
+ * NaN.  Sequences of one call share no block that it writes.  lengths[s] is at
+ * least the rows of sequence s; rows ahead of position 0 are padding too. */
 int kvsnap_append(const kvsnap_paged_layer* layer, const kvsnap_sequences* sequences, const kvsnap_rotation* rotation,
                   const void* key, int64_t key_token_stride, int64_t key_head_stride, const void* value,
                   int64_t value_token_stride, int64_t value_head_stride, const void* query, int64_t query_token_stride,
@@ -113,10 +114,10 @@ size_t kvsnap_attend_workspace_bytes(const kvsnap_paged_layer* layer, int64_t to
 /* out[row, h] = the sum over the tokens t that a row sees of softmax(scale *
  * query[row, h] . key[t]) value[t], for query and out of `tokens` rows of
  * `heads` heads (a multiple of the layer's, consecutive ones sharing a key
- * head) of type bf16 or fp16; a 16-bit cache is of the same type.  The row at
- * position p of its sequence sees tokens 0..p, with window > 0 the last
- * `window` of them; one that sees none, or scores of -inf alone, has
- * zeros and a log sum of -inf.
+ * head) of type bf16 or fp16; a 16-bit cache is of the same type, and out may
+ * be query, but otherwise overlaps no part of it.  The row at position p of its
+ * sequence sees tokens 0..p, with window > 0 the last `window` of them; one
+ * that sees none, or scores of -inf alone, has zeros and a log sum of -inf.
  * Softmax, sums and products' sums are fp32; weights are rounded to 16 bits
  * before they meet the values (to two such terms for fp16 queries over an
  * e4m3 cache; an fp16 cache's by at least 2^-30 of the largest weight among

@@ -67,7 +67,8 @@ def rotate(x, positions, rotary, *, axes=None, interleaved=False, inverse=False,
     are copied.  ``positions`` (int64 or int32) is ``[tokens]``, or ``[axes, tokens]`` for positions of several axes
     (time, height and width, say), where ``axes`` names the axis of each pair.  A position outside ``rotary``'s rows
     has no angle and gives NaN.  ``inverse`` turns the other way: it undoes a rotation, gives its gradient, and moves
-    kept keys to earlier positions.  ``out`` (a new tensor if None) may be ``x`` itself.
+    kept keys to earlier positions.  ``out`` (a new tensor if None) may be ``x`` itself, and otherwise overlaps no part
+    of it.
     """
     return attention_binding().rotate(x, positions, rotary, axes, interleaved, inverse, out)
 
@@ -132,7 +133,8 @@ class PagedCache:
                axes=None, interleaved=False, query_out=None):
         """Put a step's ``key`` and ``value`` ([rows, heads, width], bfloat16 or float16) into the slots of their
         sequences' last tokens, in one launch, and return ``query`` ([rows, query heads, width]) turned like the keys
-        (into ``query_out`` if given, which may be ``query``; None without a query).
+        (into ``query_out`` if given, which may be ``query`` and otherwise overlaps nothing that is read; None without a
+        query).
 
         With ``rotary`` keys and queries are turned by ``positions`` as :func:`rotate` does; without positions a
         token's is its place in its sequence.  A 16-bit cache must have the keys' type.  Into an e4m3 cache a block's
@@ -148,7 +150,7 @@ class PagedCache:
                window=None, out=None, return_lse=False):
         """Attention of a step's ``query`` rows ([rows, query heads, width], bfloat16 or float16) over their
         sequences' tokens in the cache, the step's own included: ``[rows, query heads, width]`` of the query's type
-        (``out`` if given).
+        (``out`` if given, which may be ``query`` and otherwise overlaps no part of it).
 
         Query heads are a multiple of the cache's; consecutive ones share a key head.  A row at position p sees the
         tokens 0 to p of its sequence, with ``window`` the last ``window`` of them, itself among them; a row that

@@ -252,6 +252,50 @@ at::Tensor output(PyObject* object, const char* what, at::IntArrayRef sizes, con
     return out;
 }
 
+// Whether two [tokens, heads, width] tensors share memory.  Where their ranges meet, they are apart if along an axis of
+// one stride each lies in its own part of every period (heads of one projection), or, with both strides alike, in its own
+// part of every inner one.
+bool meet(const at::Tensor& a, const at::Tensor& b) {
+    struct Places {
+        int64_t first, size[2], stride[2], width;
+        explicit Places(const at::Tensor& t)
+            : first(reinterpret_cast<intptr_t>(t.data_ptr())), size{t.size(0), t.size(1)},
+              stride{t.stride(0) * t.element_size(), t.stride(1) * t.element_size()},
+              width(t.size(2) * t.element_size()) {}
+        int64_t extent(int axis) const { return (size[axis] - 1) * stride[axis] + width; }
+        int64_t end() const { return first + (size[0] - 1) * stride[0] + extent(1); }
+    };
+    if (a.numel() == 0 || b.numel() == 0) return false;
+    const Places x(a), y(b);
+    if (x.end() <= y.first || y.end() <= x.first) return false;
+    const auto period = [&](int axis) -> int64_t {          // the stride of both, 0 if they differ
+        const int64_t of = x.size[axis] > 1 ? x.stride[axis] : y.stride[axis];
+        return (x.size[axis] > 1 && x.stride[axis] != of) || (y.size[axis] > 1 && y.stride[axis] != of) ? 0 : of;
+    };
+    const auto apart = [&](int64_t each, int64_t x_extent, int64_t y_extent) {
+        const int64_t at = ((y.first - x.first) % each + each) % each;
+        return at >= x_extent && at + y_extent <= each;
+    };
+    for (const int axis : {0, 1})
+        if (period(axis) > 0 && apart(period(axis), x.extent(1 - axis), y.extent(1 - axis))) return false;
+    const int64_t outer = std::max(period(0), period(1)), inner = std::min(period(0), period(1));
+    return !(inner > 0 && outer % inner == 0 && apart(inner, x.width, y.width));
+}
+
+bool same_places(const at::Tensor& a, const at::Tensor& b) {
+    bool same = a.data_ptr() == b.data_ptr() && a.sizes() == b.sizes();
+    for (int64_t axis = 0; same && axis < a.dim(); ++axis) same = a.size(axis) <= 1 || a.stride(axis) == b.stride(axis);
+    return same;
+}
+
+// Rows are read while others are written: a given output is the rows it is made from, or apart from them.
+void check_apart(PyObject* object, const at::Tensor& out, const char* what, const at::Tensor& from, const char* name,
+                 bool itself) {
+    if (!given(object) || (itself && same_places(out, from)) || !meet(out, from)) return;
+    if (itself) refuse(what, " must be ", name, " itself or not overlap it");
+    refuse(what, " must not overlap ", name);
+}
+
 // ----------------------------------------------------------------- calls
 
 // bind(rotate, append, attend, attend_workspace_bytes, cuda_error): the entry points' addresses.
@@ -280,6 +324,7 @@ PyObject* rotate(PyObject*, PyObject* const* args, Py_ssize_t count) {
         if (!given(args[1]) || !given(args[2])) refuse("a rotation needs positions and a rotary table");
         const Rotation r = rotation_of(args[2], args[1], args[3], truth(args[4]), truth(args[5]), tokens, width);
         const at::Tensor out = output(args[6], "out", {tokens, heads, width}, x);
+        check_apart(args[6], out, "out", x, "x", true);
         check_device(x.device(), {&out, r.table, r.positions});
         launched(x.device(), [&](uintptr_t stream) {
             return library.rotate(x.data_ptr(), x.stride(0), x.stride(1), out.data_ptr(), out.stride(0),
@@ -324,6 +369,9 @@ PyObject* append(PyObject*, PyObject* const* args, Py_ssize_t count) {
             check_rows(*query, "query", tokens, -1, width);
             if (query->scalar_type() != key.scalar_type()) refuse("query must have the keys' type");
             out = output(args[12], "query_out", query->sizes(), *query);
+            check_apart(args[12], out, "query_out", *query, "query", true);
+            check_apart(args[12], out, "query_out", key, "key", false);
+            check_apart(args[12], out, "query_out", value, "value", false);
         } else if (given(args[12])) {
             refuse("query_out needs a query");
         }
@@ -377,6 +425,7 @@ PyObject* attend(PyObject*, PyObject* const* args, Py_ssize_t count) {
             if (longest < 0) refuse("max_length must not be negative");
         }
         const at::Tensor out = output(args[9], "out", query.sizes(), query);
+        check_apart(args[9], out, "out", query, "query", true);
         const bool wants_lse = truth(args[10]);
         check_device(layer.device, {&query, &out, s.tables, s.lengths, s.starts});
         at::Tensor lse, scratch;

@@ -120,3 +120,42 @@ def test_a_rotary_table_of_no_positions_is_refused():
         append(layer(), step(), rotary=none)
     with pytest.raises(ValueError, match="of one position or more"):
         rotate(torch.zeros((3, 2, 64)), torch.zeros(3, dtype=torch.int64), none)
+
+
+FUSED = torch.zeros((5, 12, 64), dtype=torch.bfloat16)
+WIDE = torch.zeros((5, 4, 3, 64), dtype=torch.bfloat16)             # a head's query, key and value side by side
+
+
+@pytest.mark.parametrize("out,overlaps", [
+    (FUSED[:3, 0:4], False),                    # query itself
+    (FUSED[:3, 4:8], False), (FUSED[:3, 8:12], False), (FUSED[3:5].reshape(-1)[:768].view(3, 4, 64), False),
+    (FUSED[:3, 1:5], True), (FUSED[:3, 3:7], True), (FUSED[1:4, 0:4], True), (FUSED[2:5, 0:4], True),
+    (FUSED.view(-1)[:768].view(3, 4, 64), True), (FUSED.view(-1)[512:1280].view(3, 4, 64), True),
+    (FUSED.view(-1)[8:].as_strided((3, 4, 64), (768, 64, 1), 8), True),
+    (FUSED.view(-1).as_strided((3, 4, 64), (64, 192, 1), 0), True),
+    (torch.zeros((3, 4, 64), dtype=torch.bfloat16), False),
+])
+def test_an_output_over_other_rows_of_its_input_is_refused(out, overlaps):
+    query = FUSED[:3, 0:4]
+    why = "itself or not overlap it" if overlaps else ON_CPU
+    positions, table = torch.zeros(3, dtype=torch.int64), torch.zeros((5, 32, 2))
+    with pytest.raises(ValueError, match=why):
+        rotate(query, positions, table, out=out)
+    with pytest.raises(ValueError, match=why):
+        append(layer(), step(), query=query, query_out=out)
+    with pytest.raises(ValueError, match=why):
+        attend(layer(), step(), query=query, out=out)
+
+
+def test_an_output_over_keys_or_values_is_refused():
+    q, k, v = FUSED[:3].split([4, 4, 4], 1)
+    append_to = layer(kv=4)
+    for out, why in ((q, ON_CPU), (k, "query_out must not overlap key"), (v, "query_out must not overlap value"),
+                     (FUSED[:3, 2:6], "query itself or not overlap it"), (FUSED[:3, 6:10], "must not overlap key")):
+        with pytest.raises(ValueError, match=why):
+            append(append_to, step(kv=4), query=q, key=k, value=v, query_out=out)
+    q, k, v = WIDE[:3].unbind(2)
+    for out, why in ((q, ON_CPU), (k, "query_out must not overlap key"), (v, "query_out must not overlap value"),
+                     (WIDE[2:5, :, 0], "query itself or not overlap it"), (WIDE[2:5, :, 1], "must not overlap key")):
+        with pytest.raises(ValueError, match=why):
+            append(append_to, step(kv=4), query=q, key=k, value=v, query_out=out)

@@ -8,7 +8,7 @@ torch = pytest.importorskip("torch")
 
 from kvsnap_amd.attention import PagedCache, block_scales
 from paged_reference import E4M3, attend64, dequantised
-from test_gpu_attend import check, made
+from test_gpu_attend import check, made, make, tables_for
 
 pytestmark = [pytest.mark.gpu, pytest.mark.usefixtures("hip_library")]
 
@@ -107,3 +107,22 @@ def test_small_weights_behind_one_that_takes_all_in_fp16(sink, rows):
     off = (got.cpu().double() - want).abs() - bound
     assert off.max() <= 0, (off.amax((0, 2)) / want.amin((0, 2))).tolist()
     assert ((lse.cpu().double() - want_lse).abs() <= 2.0 ** -12 + 2.0 ** -22 * want_lse.abs()).all()
+
+
+@pytest.mark.parametrize("added,lengths", [([1, 1, 1], [40, 0, 300]), ([1, 1, 1], [3000, 17, 900]), ([300], [300]),
+                                           ([3, 1, 40, 1], [2800, 1500, 90, 7])])
+def test_queries_that_become_their_own_output(added, lengths):
+    """Whole and cut, rows alone and in tiles: ``out`` is ``query``, heads of a projection."""
+    blocks = sum(-(-n // 16) for n in lengths) + 2
+    layer, _ = make("kv_split", blocks, 16, 2, 64, BF16, 3)
+    tables = tables_for(lengths, 16, blocks, 3).cuda()
+    lengths = torch.tensor(lengths, dtype=torch.int32).cuda()
+    starts = torch.tensor([sum(added[:s]) for s in range(len(added) + 1)], dtype=torch.int32).cuda()
+    fused = made((sum(added), 12, 64), BF16, 4).cuda()
+    query = fused[:, 2:10]
+    starts = None if max(added) == 1 else starts
+    want = layer.attend(query, tables, lengths, query_starts=starts)
+    before = fused.clone()
+    assert layer.attend(query, tables, lengths, query_starts=starts, out=query) is query
+    assert torch.equal(query, want)
+    assert torch.equal(fused[:, :2], before[:, :2]) and torch.equal(fused[:, 10:], before[:, 10:])

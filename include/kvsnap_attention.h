@@ -27,7 +27,7 @@
  * token lengths[s] - (query_starts[s + 1] - query_starts[s]) + i of sequence
  * s (query_starts: n_seqs + 1 int32, rising from 0); without query_starts
  * every sequence has one row, row s.  Rows past the last sequence's are
- * padding: nothing is read for them and nothing written.  These tables are
+ * padding: they may be read, but nothing is written for them.  These tables are
  * read on the device and may change between replays of a captured launch.  A
  * table entry outside [0, blocks) names no block: nothing is written for it
  * and its tokens are seen by nobody; so are tokens past the table's width.
@@ -64,7 +64,7 @@ typedef struct kvsnap_sequences {
 } kvsnap_sequences;
 
 /* Positions and angles.  angles: fp32 [rows, pairs, 2], the cosine and sine
- * of pair j at each position (8-byte aligned); pairs is a multiple of 8.
+ * of pair j at each position (16-byte aligned); pairs is a multiple of 8.
  * Pair j turns values j and j + pairs of a head, or 2j and 2j + 1 where
  * `interleaved`; values from 2 * pairs on are left as they are.  positions:
  * int64 (or int32 where `narrow`), axis_stride apart for each axis; axes[u]
@@ -97,8 +97,9 @@ int kvsnap_rotate(const void* x, int64_t x_token_stride, int64_t x_head_stride, 
  * slots filled before this step need more; where the new ones do, the slots
  * before them are rounded again to the new scale.  Slots past the sequence's
  * length are left as they are, and a value that is not finite is stored as
- * NaN.  Sequences of one call share no block that it writes.  lengths[s] is at
- * least the rows of sequence s; rows ahead of position 0 are padding too. */
+ * NaN.  No block that a call writes is named twice by the pages that it writes, of
+ * one sequence or of several.  lengths[s] is at least the rows of sequence s;
+ * rows ahead of position 0 are padding too. */
 int kvsnap_append(const kvsnap_paged_layer* layer, const kvsnap_sequences* sequences, const kvsnap_rotation* rotation,
                   const void* key, int64_t key_token_stride, int64_t key_head_stride, const void* value,
                   int64_t value_token_stride, int64_t value_head_stride, const void* query, int64_t query_token_stride,
@@ -120,9 +121,11 @@ size_t kvsnap_attend_workspace_bytes(const kvsnap_paged_layer* layer, int64_t to
  * that sees none, or scores of -inf alone, has zeros and a log sum of -inf.
  * Softmax, sums and products' sums are fp32; weights are rounded to 16 bits
  * before they meet the values (to two such terms for fp16 queries over an
- * e4m3 cache; an fp16 cache's by at least 2^-30 of the largest weight among
- * 64 tokens, which moves an output by at most 2^-24 of the largest value),
- * and an e4m3 cache's values are exact in bf16.  lse, or NULL:
+ * e4m3 cache; over an fp16 cache what is under 2^-30 of the largest among 64
+ * tokens may vanish, which moves an output by at most 2^-24 of the largest
+ * value), and an e4m3 cache's values are exact in bf16 at scales from 2^-117 to
+ * 2^119 (past them, what is under 2^-126 may vanish and what is over bf16's largest
+ * is infinite).  lse, or NULL:
  * fp32 [tokens, heads], the natural logarithm of each row's sum of
  * exponentials.  max_length, at least every sequence's length if it can be
  * known, only shapes the launch.  workspace: 16-byte aligned scratch of

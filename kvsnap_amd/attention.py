@@ -141,7 +141,8 @@ class PagedCache:
         new values go by the least power of two that keeps them within e4m3's range, or by the block's own where
         slots filled before need more; where the new ones need more, the filled slots are rounded again.  Values that
         are not finite are stored as NaN.  Slots past the length stay as they are, and so do the rows of
-        ``query_out`` that are padding.  Sequences of one call must not share a block that it writes.
+        ``query_out`` that are padding (in a new tensor they hold anything).  The pages that one call writes must name
+        a block only once, in one sequence and in all of them.
         """
         return self._call.append(self._layer_at, self.cache, key, value, block_tables, lengths, query_starts, query,
                                  positions, rotary, axes, interleaved, query_out)
@@ -155,7 +156,7 @@ class PagedCache:
         Query heads are a multiple of the cache's; consecutive ones share a key head.  A row at position p sees the
         tokens 0 to p of its sequence, with ``window`` the last ``window`` of them, itself among them; a row that
         sees none (a sequence of length 0), or scores of -inf alone, gets zeros, and rows of ``out`` that are padding
-        stay as they are.  Scores are ``softmax_scale`` (``width ** -0.5`` if None)
+        stay as they are (in a new tensor, and in ``lse``, they hold anything).  Scores are ``softmax_scale`` (``width ** -0.5`` if None)
         times the products; softmax and sums are fp32.  A 16-bit cache must have the query's type.
 
         ``max_length``, the longest sequence's length if the caller knows it (the tables' width if None), only shapes

@@ -47,7 +47,8 @@ struct Matrix<_Float16> {
 };
 
 // What the products run in: the cache's 16-bit type, or bf16 for an e4m3 cache, whose every value times its block's
-// power of two is a bf16.  fp16 queries and weights are then two bf16 terms each, their first and the rest: 16 bits of
+// power of two is a bf16 (from 2^-117 to 2^119; the bits of e4m3's least values fall out below, its largest are infinite
+// above).  fp16 queries and weights are then two bf16 terms each, their first and the rest: 16 bits of
 // the value, where one bf16 would lose three of fp16's.
 template <typename Q, bool kEight>
 struct Shape {

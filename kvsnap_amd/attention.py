@@ -80,7 +80,8 @@ class PagedCache:
     K/V-split ``[2, blocks, tokens, heads, width]`` tensor of ``block_size`` token slots a block, in bfloat16,
     float16 or float8_e4m3fn; widths are multiples of 16 up to 256.  An e4m3 cache comes with ``scales``
     (float8_e8m0fnu or uint8 ``[blocks, heads, 2]``, K's and V's, see :func:`block_scales`): a stored value stands
-    for itself times its block and head's power of two.  The cache is kept, not copied.
+    for itself times its block and head's power of two (to be appended to, a byte of its own).  The cache is kept,
+    not copied.
 
     Every call takes the step's tables (int32, on the cache's device, read there): ``block_tables`` ``[sequences,
     most blocks]``, ``lengths`` ``[sequences]`` counting the step's own tokens, and ``query_starts`` ``[sequences +
@@ -112,7 +113,7 @@ class PagedCache:
             raise ValueError("a paged cache's rows must be 16-byte aligned")
         if (scales is not None) != (kind == 2):
             raise ValueError("an e4m3 cache needs scales, and no other takes them")
-        scale_strides = (0, 0, 0)
+        scale_strides, self._shared = (0, 0, 0), False
         if scales is not None:
             if str(scales.dtype) not in ("torch.float8_e8m0fnu", "torch.uint8") or (
                     tuple(scales.shape) != (blocks, heads, 2)):
@@ -121,6 +122,11 @@ class PagedCache:
             if scales.device != cache.device:
                 raise ValueError("a cache's scales must be on its device")
             scale_strides = scales.stride()
+            covered = 0         # by the nearer axes: each block, head and side needs a byte of its own to be appended
+            for stride, count in sorted(zip(scale_strides, scales.shape)):
+                if count > 1:
+                    self._shared = self._shared or stride <= covered
+                    covered += (count - 1) * stride
         self.cache, self.scales, self.block_size = cache, scales, block_size
         self.blocks, self.heads, self.width, self.device = blocks, heads, width, cache.device
         self._kind = kind
@@ -144,6 +150,8 @@ class PagedCache:
         ``query_out`` that are padding (in a new tensor they hold anything).  The pages that one call writes must name
         a block only once, in one sequence and in all of them.
         """
+        if self._shared:
+            raise ValueError("the cache's scales share bytes among blocks, heads or K and V: none can be appended to")
         return self._call.append(self._layer_at, self.cache, key, value, block_tables, lengths, query_starts, query,
                                  positions, rotary, axes, interleaved, query_out)
 
@@ -156,8 +164,8 @@ class PagedCache:
         Query heads are a multiple of the cache's; consecutive ones share a key head.  A row at position p sees the
         tokens 0 to p of its sequence, with ``window`` the last ``window`` of them, itself among them; a row that
         sees none (a sequence of length 0), or scores of -inf alone, gets zeros, and rows of ``out`` that are padding
-        stay as they are (in a new tensor, and in ``lse``, they hold anything).  Scores are ``softmax_scale`` (``width ** -0.5`` if None)
-        times the products; softmax and sums are fp32.  A 16-bit cache must have the query's type.
+        stay as they are (in a new tensor, and in ``lse``, they hold anything).  Scores are
+        ``softmax_scale`` (``width ** -0.5`` if None) times the products; softmax and sums are fp32.  A 16-bit cache must have the query's type.
 
         ``max_length``, the longest sequence's length if the caller knows it (the tables' width if None), only shapes
         the launch.  With ``return_lse`` the result is ``(out, lse)``: fp32 ``[rows, query heads]`` natural

@@ -159,3 +159,21 @@ def test_an_output_over_keys_or_values_is_refused():
                      (WIDE[2:5, :, 0], "query itself or not overlap it"), (WIDE[2:5, :, 1], "must not overlap key")):
         with pytest.raises(ValueError, match=why):
             append(append_to, step(kv=4), query=q, key=k, value=v, query_out=out)
+
+
+@pytest.mark.parametrize("scales,shared", [
+    (torch.zeros((4, 1, 1), dtype=torch.uint8).expand(4, 2, 2), True),           # one a block, broadcast
+    (torch.zeros((1, 2, 2), dtype=torch.uint8).expand(4, 2, 2), True),
+    (torch.zeros((4, 2, 1), dtype=torch.uint8).expand(4, 2, 2), True),
+    (torch.zeros((20,), dtype=torch.uint8).as_strided((4, 2, 2), (2, 1, 1)), True),
+    (torch.zeros((20,), dtype=torch.uint8).as_strided((4, 2, 2), (3, 2, 1)), True),
+    (torch.zeros((2, 4, 2), dtype=torch.uint8).transpose(0, 1), False),
+    (torch.zeros((2, 2, 4), dtype=torch.uint8).permute(2, 1, 0), False),
+    (block_scales(4, 3, 2)[1][1], False),
+])
+def test_scales_that_share_bytes_are_read_but_not_appended_to(scales, shared):
+    held = PagedCache(torch.zeros((2, 4, 16, 2, 64)).to(torch.float8_e4m3fn), 16, scales=scales)
+    with pytest.raises(ValueError, match="share bytes" if shared else ON_CPU):
+        append(held, step())
+    with pytest.raises(ValueError, match=ON_CPU):
+        attend(held, step())

@@ -165,7 +165,8 @@ class PagedCache:
         tokens 0 to p of its sequence, with ``window`` the last ``window`` of them, itself among them; a row that
         sees none (a sequence of length 0), or scores of -inf alone, gets zeros, and rows of ``out`` that are padding
         stay as they are (in a new tensor, and in ``lse``, they hold anything).  Scores are
-        ``softmax_scale`` (``width ** -0.5`` if None) times the products; softmax and sums are fp32.  A 16-bit cache must have the query's type.
+        ``softmax_scale`` (``width ** -0.5`` if None) times the products; softmax and sums are fp32.  A 16-bit cache
+        must have the query's type.
 
         ``max_length``, the longest sequence's length if the caller knows it (the tables' width if None), only shapes
         the launch.  With ``return_lse`` the result is ``(out, lse)``: fp32 ``[rows, query heads]`` natural

@@ -296,6 +296,12 @@ void check_apart(PyObject* object, const at::Tensor& out, const char* what, cons
     refuse(what, " must not overlap ", name);
 }
 
+// Tells autograd that a tensor's values changed, as torch's own in-place operators do: a graph that saved it must not
+// use them.
+void written(const at::Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // ----------------------------------------------------------------- calls
 
 // bind(rotate, append, attend, attend_workspace_bytes, cuda_error): the entry points' addresses.
@@ -331,6 +337,7 @@ PyObject* rotate(PyObject*, PyObject* const* args, Py_ssize_t count) {
                                   out.stride(1), tokens, static_cast<int>(heads), static_cast<int>(width), type,
                                   &r.raw, stream);
         });
+        if (given(args[6])) written(out);
         return THPVariable_Wrap(out);
     });
 }
@@ -385,6 +392,8 @@ PyObject* append(PyObject*, PyObject* const* args, Py_ssize_t count) {
                                   query ? out.stride(0) : 0, query ? out.stride(1) : 0, tokens,
                                   query ? static_cast<int>(query->size(1)) : 0, type, stream);
         });
+        written(THPVariable_Unpack(args[1]));
+        if (given(args[12])) written(out);
         if (!query) Py_RETURN_NONE;
         return THPVariable_Wrap(out);
     });
@@ -440,6 +449,7 @@ PyObject* attend(PyObject*, PyObject* const* args, Py_ssize_t count) {
                                   static_cast<float>(scale), window, longest, size ? scratch.data_ptr() : nullptr,
                                   size, stream);
         });
+        if (given(args[9])) written(out);
         if (!wants_lse) return THPVariable_Wrap(out);
         PyObject* const first = THPVariable_Wrap(out);
         PyObject* const second = THPVariable_Wrap(lse);

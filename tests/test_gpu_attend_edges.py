@@ -6,7 +6,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
-from kvsnap_amd.attention import PagedCache, block_scales
+from kvsnap_amd.attention import PagedCache, rotary_table, rotate
 from paged_reference import E4M3, attend64, dequantised
 from test_gpu_attend import check, made, make, tables_for
 
@@ -126,3 +126,30 @@ def test_queries_that_become_their_own_output(added, lengths):
     assert layer.attend(query, tables, lengths, query_starts=starts, out=query) is query
     assert torch.equal(query, want)
     assert torch.equal(fused[:, :2], before[:, :2]) and torch.equal(fused[:, 10:], before[:, 10:])
+
+
+def test_a_graph_that_saved_what_a_call_writes_does_not_use_it():
+    """Backward through a tensor that was written since raises, as after torch's own in-place operators; inference
+    tensors, which have no version, are written all the same."""
+    layer, _ = make("kv_split", 4, 16, 2, 64, BF16, 1)
+    tables = torch.tensor([[1, 2]], dtype=torch.int32, device="cuda")
+    lengths = torch.tensor([20], dtype=torch.int32, device="cuda")
+    angles = rotary_table(64, 30, device="cuda")
+    at = torch.tensor([3], device="cuda")
+    query, key = made((1, 4, 64), BF16, 2).cuda(), made((1, 2, 64), BF16, 3).cuda()
+    calls = [(lambda out: rotate(query, at, angles, out=out), torch.empty_like(query)),
+             (lambda out: layer.append(key, key, tables, lengths, query=query, query_out=out), torch.empty_like(query)),
+             (lambda out: layer.attend(query, tables, lengths, out=out), torch.empty_like(query)),
+             (lambda out: layer.append(key, key, tables, lengths), layer.cache)]
+    for call, out in calls:
+        weight = torch.ones((), dtype=BF16, device="cuda", requires_grad=True)
+        product = (weight * out).sum()
+        call(out)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            product.backward()
+        if out is not layer.cache:
+            want = out.clone()
+            with torch.inference_mode():
+                again = torch.zeros_like(out)
+                call(again)
+            assert torch.equal(again, want)

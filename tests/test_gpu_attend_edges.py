@@ -153,3 +153,77 @@ def test_a_graph_that_saved_what_a_call_writes_does_not_use_it():
                 again = torch.zeros_like(out)
                 call(again)
             assert torch.equal(again, want)
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+@pytest.mark.parametrize("size", [16, 24])
+@pytest.mark.parametrize("byte", [0, 1, 240])
+def test_e8m0_bytes_at_their_ends_in_rows_and_tiles(byte, size, rows):
+    """V's scales at 2^-127, 2^-126 and 2^113, weights all alike: the mean of what a row sees, one rounding of the
+    weights and one of the output, and what is under bf16's least normal number may vanish."""
+    layer, _ = make("kv_split", 12, size, 1, 64, E4M3, 9)
+    held = layer.scales.view(torch.uint8)
+    held[..., 0], held[..., 1] = 127, byte
+    exact = dequantised(layer.cache.cpu(), layer.scales.cpu())
+    length = 12 * size - 5
+    tables, lengths = tables_for([length], size, 12, 4, spare=0), torch.tensor([length], dtype=torch.int32)
+    starts = torch.tensor([0, rows], dtype=torch.int32)
+    query = torch.zeros((rows, 2, 64), dtype=BF16)
+    got = layer.attend(query.cuda(), tables.cuda(), lengths.cuda(), query_starts=starts.cuda()).cpu().double()
+    want, _ = attend64(query, *exact, tables, lengths, starts)
+    spread, _ = attend64(query, exact[0], exact[1].abs(), tables, lengths, starts)
+    assert ((got - want).abs() <= (2.0 ** -8 + 2.0 ** -12) * spread + 2.0 ** -8 * want.abs() + 2.0 ** -126).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("side", [0, 1])
+@pytest.mark.parametrize("size", [16, 24])
+def test_a_scale_that_is_nan_reaches_the_rows_that_see_its_block(size, side, dtype):
+    """The byte 255, of K or of V, in the last block, which the last 11 of 60 rows see, and in a block in the middle
+    that only a window's first rows do."""
+    layer, _ = make("kv_split", 14, size, 2, 64, E4M3, 9)
+    length, rows = 12 * size + 11, 60
+    tables = tables_for([length], size, 14, 4).cuda()
+    lengths = torch.tensor([length], dtype=torch.int32, device="cuda")
+    starts = torch.tensor([0, rows], dtype=torch.int32, device="cuda")
+    query = made((rows, 4, 64), dtype, 5).cuda()
+    held = layer.scales.view(torch.uint8)
+    clean = layer.attend(query, tables, lengths, query_starts=starts)
+    block = int(tables[0, 12])
+    before = held[block, 0, side].clone()
+    held[block, 0, side] = 255                                  # head 0's; head 1's is as it was
+    got = layer.attend(query, tables, lengths, query_starts=starts)
+    assert got[rows - 11:, :2].isnan().all()
+    assert torch.equal(got[:rows - 11], clean[:rows - 11]) and torch.equal(got[:, 2:], clean[:, 2:])
+    assert layer.attend(query[-1:], tables, lengths)[:, :2].isnan().all()
+    held[block, 0, side] = before
+    # a window of 50: the first row sees from length - 60 - 49 on, and the block of that token to its end
+    window, first = 50, length - rows + 1 - 50
+    clean = layer.attend(query, tables, lengths, query_starts=starts, window=window)
+    page = first // size
+    held[int(tables[0, page]), 1, side] = 255
+    got = layer.attend(query, tables, lengths, query_starts=starts, window=window)
+    seen = (page + 1) * size - first                            # rows that see its last token
+    assert got[:seen, 2:].isnan().all()
+    assert torch.equal(got[seen:], clean[seen:]) and torch.equal(got[:, :2], clean[:, :2])
+
+
+@pytest.mark.parametrize("held", ["16-bit", "e4m3"])
+@pytest.mark.parametrize("size", [16, 24, 1])
+@pytest.mark.parametrize("width", [80, 96, 112, 128, 192, 256])
+def test_cut_rows_and_tiles_of_every_width(width, size, held):
+    """Parts joined where a head's quarter does not divide a workgroup, at the widest, and over blocks that are no whole
+    groups of 16 tokens: single rows and chunks over long contexts, in one step and each alone, with a window too."""
+    lengths = [2900, 33, 1500, 700]
+    blocks = sum(-(-n // size) for n in lengths) + 1
+    layer, exact = make("kv_split", blocks, size, 2, width, E4M3 if held == "e4m3" else FP16, width)
+    tables, dtype = tables_for(lengths, size, blocks, width), FP16
+    lengths = torch.tensor(lengths, dtype=torch.int32)
+    for added, window in (([1, 1, 1, 1], None), ([1, 3, 30, 1], None), ([2, 1, 5, 40], 1400)):
+        starts = torch.tensor([sum(added[:s]) for s in range(5)], dtype=torch.int32)
+        if max(added) == 1:
+            starts = None
+        query = made((sum(added), 6, width), dtype, 7)
+        out, lse = layer.attend(query.cuda(), tables.cuda(), lengths.cuda(), window=window, return_lse=True,
+                                query_starts=None if starts is None else starts.cuda())
+        check(out, query, exact, tables, lengths, starts, lse=lse, window=window)

@@ -82,7 +82,8 @@ struct Weights {
     float factor, slack, fall;
 
     __device__ __forceinline__ Weights(float factor, float slack_of)
-        : factor(factor), slack(__builtin_fminf(slack_of / factor, 1e30f)), fall(__builtin_fminf(kFall / factor, 1e30f)) {}
+        : factor(factor), slack(slack_of > 0 ? __builtin_fminf(slack_of / factor, 1e30f) : 0),
+          fall(__builtin_fminf(kFall / factor, 1e30f)) {}
 
     // Whether a row's reference moves for scores of at most `most`, and where to.  Down no farther than sums of `total`,
     // the row's, have room to grow: to 2^90, and values are at most 2^16.
@@ -149,10 +150,11 @@ __device__ __forceinline__ float sum_across_halves(float x) {
     return bits<float>(halves[0]) + bits<float>(halves[1]);
 }
 
-// Weights are 2^(score * factor - top * factor), rounded once behind the second product.  What rounding that product
-// moves is common to a row's weights and falls out, while it is little: whether some row's is more than 2^-14 (largest
-// scores from some 2^10 binary logarithms on).  There scores are taken less `top` before they meet the factor: exact
-// for the tokens that count, and never a power that overflows or leaves every weight 0.
+// Weights are 2^((score - top) * factor): the difference is exact for the tokens that count, however large the scores.
+// Rows alone take it so.  Tiles, which are short of vector instructions, take 2^(score * factor - top * factor) by one
+// operation a score: what rounding top * factor moves is common to a row's weights and falls out, while it is little.
+// Whether some row's is more than 2^-14 (largest scores from some 2^10 binary logarithms on; from some 2^30 the powers
+// overflow, or leave every weight 0) and tiles take the difference first too.
 __device__ __forceinline__ bool rounds_far(float top, float factor) {
     return __ballot(!(__builtin_fabsf(__builtin_fmaf(top, factor, -(top * factor))) <= 0x1p-14f) &&
                     top != -__builtin_inff()) != 0;
@@ -347,6 +349,13 @@ struct Tile {
     float k_scale[2], v_scale[2][4];                        // e4m3 only
 };
 
+// Waves of a SIMD that attend_row_kernel's registers leave room for.  Two terms over blocks that are no whole groups of
+// 16 tokens spill at four, and take 7 % longer than at two.
+template <typename Q, bool kEight, int kJ, bool kWhole>
+constexpr int row_waves() {
+    return kEight && kJ <= 8 && (kWhole || Shape<Q, kEight>::kTerms == 1) ? 4 : 2;
+}
+
 // A row's heads of `beside` key heads over one part of its tokens, a workgroup of eight waves; those of one key head take
 // its tiles of 32 tokens in turn.
 //
@@ -358,7 +367,7 @@ struct Tile {
 // the last workgroups' end.  Loads that keep out of the caches (nontemporal) are 5 % faster there and up to 45 % slower
 // where a cache fits what the chip's does.
 template <typename Q, bool kEight, int kJ, bool kWhole, bool kExact>
-__global__ __launch_bounds__(kWaves * 64, kEight && kJ <= 8 ? 4 : 2) void attend_row_kernel(Attend a) {
+__global__ __launch_bounds__(kWaves * 64, row_waves<Q, kEight, kJ, kWhole>()) void attend_row_kernel(Attend a) {
     using T = typename Shape<Q, kEight>::T;
     using Vec = typename Matrix<T>::Vec;
     using W = Weights<T>;
@@ -411,7 +420,6 @@ __global__ __launch_bounds__(kWaves * 64, kEight && kJ <= 8 ? 4 : 2) void attend
     float top = -__builtin_inff(), total = 0;
     const float factor = a.scale * kLog2e;
     const W weights(factor, W::kFollow ? 6 : 0);
-    bool far = false;
 
     const int base = (sight.low & ~(kTile - 1)) + part * job.chunk * kTile;
     const int stop = part == parts - 1 ? sight.high : min(sight.high, base + job.chunk * kTile);
@@ -563,18 +571,12 @@ __global__ __launch_bounds__(kWaves * 64, kEight && kJ <= 8 ? 4 : 2) void attend
 #pragma unroll
             for (int j = 0; j < kJ; ++j) sum[j] *= shrink;
             top = to;
-            far = rounds_far(top, factor);
         }
-        float against = top == -__builtin_inff() ? 0.0f : __builtin_fmaf(top, factor, -W::kLift);
-        if (far) {
-#pragma unroll
-            for (int t = 0; t < 8; ++t) score[t >> 2][t & 3] -= top == -__builtin_inff() ? 0.0f : top;
-            against = -W::kLift;
-        }
+        const float from = top == -__builtin_inff() ? 0.0f : top;
         Vec p[kTerms];
 #pragma unroll
         for (int t = 0; t < 8; ++t) {
-            const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(score[t >> 2][t & 3], factor, -against));
+            const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(score[t >> 2][t & 3] - from, factor, W::kLift));
             total += x;
             if constexpr (kTerms == 2) two_terms(x, p[0], p[1], t);
             else p[0][t] = static_cast<T>(x);

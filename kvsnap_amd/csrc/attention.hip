@@ -367,7 +367,7 @@ constexpr int row_waves() {
 // the last workgroups' end.  Loads that keep out of the caches (nontemporal) are 5 % faster there and up to 45 % slower
 // where a cache fits what the chip's does.
 template <typename Q, bool kEight, int kJ, bool kWhole, bool kExact>
-__global__ __launch_bounds__(kWaves * 64, row_waves<Q, kEight, kJ, kWhole>()) void attend_row_kernel(Attend a) {
+__global__ __launch_bounds__(kWaves * 64, (row_waves<Q, kEight, kJ, kWhole>())) void attend_row_kernel(Attend a) {
     using T = typename Shape<Q, kEight>::T;
     using Vec = typename Matrix<T>::Vec;
     using W = Weights<T>;

@@ -4,8 +4,8 @@
 // A pair (a, b) of a head's values becomes (a cos - b sin, b cos + a sin) of its position's angle, in fp32 from the
 // inputs' type and rounded once, to the output's.  Nothing here is more than one pass over the data, so memory is the
 // bound: a lane takes 16 values of one head (two 16-byte loads, eight pairs, the 64 bytes of their angles), so a pair
-// never leaves its lane.  Turning 16,384 tokens of 32 heads of 128 by three axes (277 MB in and out) takes 52.4 us, 5.3 TB/s, as fast
-// as a large copy goes on this card (5.2 to 5.4).
+// never leaves its lane.  Turning 16,384 tokens of 32 heads of 128 by three axes (277 MB in and out) takes 52 us (a kernel
+// trace's), 5.3 TB/s, as fast as a large copy goes on this card (5.2 to 5.4).
 #include "launch.h"
 #include "paged.h"
 
@@ -199,8 +199,8 @@ __device__ __forceinline__ void append_query(const Step<T>& step, const kvsnap_s
 }
 
 // A 16-bit cache: each unit of a key or value to its slot, and the queries beside them in the same launch.  Two 8k prompts
-// of 32 heads over 8 of 128 (411 MB) take 84 us, 4.9 TB/s: the memory's rate for a copy, less the scattered slots.  A decode step's 0.02 to 1.5 MB
-// take 5.2 us, 4.4 of them the launch.
+// of 32 heads over 8 of 128 (411 MB) take 84 us, 4.9 TB/s: the memory's rate for a copy, less the scattered slots.  A
+// decode step's 0.02 to 1.5 MB take 5.4 us, 4.4 of them the launch.
 template <typename T>
 __global__ __launch_bounds__(kLanes) void append_kernel(Step<T> step, kvsnap_paged_layer layer, kvsnap_sequences q,
                                                         kvsnap_rotation r) {
@@ -249,8 +249,9 @@ __device__ __forceinline__ int scale_for(float top) {
 // decide, 64 / (width / 16) rows at a time.  Blocks of up to kKeep such passes (16 tokens of 128 are two) stay in
 // registers between looking for their largest value and being written; longer ones are read again.  Loads that do not
 // follow from one another are under way together: the table's entry, the rows, their angles.  Ragged chunks (3.8 MB) take
-// 12 us, a chain of loads: row starts, lengths, rows and angles, the block's scale, its filled slots (17 us with each
-// kept row loaded and turned before the next).
+// 12 us, a chain of loads: row starts, lengths, rows and angles, the block's scale, its filled slots (40 % longer with each
+// kept row loaded and turned before the next).  The last two follow from the table's entry alone, and wait behind the
+// rows' largest value only because they are asked for there.  Two 8k prompts (377 MB) take 91 us, 4.1 TB/s.
 template <typename T, int kKeep>
 __global__ __launch_bounds__(kLanes) void append_e4m3_kernel(Step<T> step, kvsnap_paged_layer layer,
                                                              kvsnap_sequences q, kvsnap_rotation r) {

@@ -362,10 +362,10 @@ constexpr int row_waves() {
 // Bound by reading K and V once: 16 query rows of a product are used for `group` heads, a quarter of them for groups
 // of four, and the matrix cores still wait for memory.  Loads go straight to the registers that the products take, as no
 // wave shares them; sixteen waves a CU are what hides their latency (a tile's loads ahead of their use, at eight waves,
-// measured the same).  64 ragged rows over 322 MB of e4m3 take 67 us, 4.8 TB/s where a plain read of as much reaches 6.6,
-// and 6 for the join; what is missing is the start, four loads that follow from one another (length, table, rows), and
-// the last workgroups' end.  Loads that keep out of the caches (nontemporal) are 5 % faster there and up to 45 % slower
-// where a cache fits what the chip's does.
+// measured the same).  64 ragged rows over 322 MB of e4m3 take 68 us (a kernel trace's), 4.8 TB/s where a plain read of
+// as much reaches 6.6, and 7 for the join; what is missing is the start, four loads that follow from one another (length,
+// table, rows), and the last workgroups' end.  Loads that keep out of the caches (nontemporal) are 5 % faster there and
+// up to 45 % slower where a cache fits what the chip's does.
 template <typename Q, bool kEight, int kJ, bool kWhole, bool kExact>
 __global__ __launch_bounds__(kWaves * 64, (row_waves<Q, kEight, kJ, kWhole>())) void attend_row_kernel(Attend a) {
     using T = typename Shape<Q, kEight>::T;
@@ -744,12 +744,12 @@ __device__ __forceinline__ uint32_t not_finite(uint32_t word) {
 // meet every bank); V's are 64 or 192 bytes past a multiple of 256, so that the 64 bytes of four rows that half a wave's
 // transposing read takes lie side by side over the banks.  No read waits for a bank.
 //
-// An 8k prompt of 32 heads over 8 of 128 in bf16 takes 615 us, 890 TFLOP/s of the products that its mask leaves, where a
+// An 8k prompt of 32 heads over 8 of 128 in bf16 takes 638 us, 861 TFLOP/s of the products that its mask leaves, where a
 // large plain product reaches 1280 on this card.  A stage costs a wave 1024 cycles of products and about 1100 of vector
 // instructions (32 scores a lane: a multiplication, an exponential, a sum, half a rounding, half a maximum), and the two
 // waves of a SIMD overlap little of the two.  Tried and slower: the next stage's scores between this stage's
-// exponentials (1004 us, not 625, at 256 registers, and 476, not 395, at width 64, where nothing spills), and higher
-// priority for waves in their products (662, not 645).
+// exponentials (1.6 times as long at 256 registers, and 1.2 times at width 64, where nothing spills), and higher priority
+// for waves in their products (3 % longer).  Widths above 128 take the registers and LDS of a whole CU: one workgroup each.
 template <typename Q, bool kEight, int kD, bool kWhole>
 __global__ __launch_bounds__(kTileWaves * 64, kD <= 128 ? 2 : 1) void attend_tile_kernel(Attend a) {
     using T = typename Shape<Q, kEight>::T;
@@ -1272,25 +1272,27 @@ struct Plan {
     int64_t row_infos = 0, tile_infos = 0, row_jobs, tile_jobs, row_parts, tile_parts;
 };
 
-// How the rows alone are cut, as measured with 32 query heads, 8 key heads of 128 and blocks of 16 tokens.
+// How the rows alone are cut, as measured with 32 query heads, 8 key heads of 128 and blocks of 16 tokens, each choice
+// against the other on one build.  Wider heads go by the same numbers.
 //
 // 8 waves side by side read a token's 8 key heads, which lie side by side, at about the same time: 64 ragged sequences
-// of up to 8k tokens in e4m3 (322 MB) take 76 us with 8 heads beside, 79 with 4 and 104 with one.  Few rows are better
-// off with all the waves on one head: the parts are joined in LDS, and one of 32k tokens takes 24.6 us, not 30.9.
+// of up to 8k tokens in e4m3 (322 MB) take 4 % longer with 4 heads beside and 37 % with one.  Few rows are better off
+// with all the waves on one head: the parts are joined in LDS, and one of 32k tokens takes 20 % less.
 constexpr int kFewHeads = 16;
-// Jobs that the sequences' tokens are cut into: in e4m3 no more than the chip holds at once (one row over 32k tokens:
-// 22.0 us; 24.8 with 450 asked for; the 64 ragged ones 76 us, 87 with 512 asked for and some 530 made).  A 16-bit cache's
-// jobs are longer, and about twice as many are better (135 us, 152 with 500; 141 with no more than 1000).
+// Jobs that the sequences' tokens are cut into: in e4m3 no more than the chip holds at once, two workgroups a CU up to
+// width 128 (one row over 32k tokens takes 13 % longer with 450 asked for, the 64 ragged ones 14 % with 512 asked for and
+// some 530 made).  A 16-bit cache's jobs are longer, and about twice as many are better (500: 12 % longer; no more than
+// 1000: 4 %).
 constexpr int kRoomE4m3 = 512, kRoom16 = 1000;
-// Tiles of a wave up to which a row is not cut, the join being 4 to 6 us, and of a part at least.
+// Tiles of a wave up to which a row is not cut, the join being 4 to 7 us, and of a part at least.
 constexpr int kWholeTurns = 5, kLeastTurns = 2;
 
-// Tiles whose jobs are fewer than the chip holds at once (two workgroups a CU) are cut into no more than it holds, where
-// that comes out: 12 sequences of up to 7700 tokens with 693 rows (16 heads over 8 of 128, e4m3) take 75 us; parts of one
-// length by the longest sequence's, as for three rounds, took 87, the last round being nearly empty.  So are up to four
-// times as many where a sequence's rows fill less than a tile, so that its tokens alone make its work: 64 sequences of up
-// to 8k tokens with 1 to 3 rows each (32 heads over 8) take 124 us, 318 whole.  A prompt's tiles are better whole, the
-// later ones first (2048 tokens: 76 us, 97 cut).
+// Tiles whose jobs are fewer than the chip holds at once (two workgroups a CU up to width 128; wider ones hold one, and
+// go in two rounds) are cut into no more than that, where it comes out: with 12 sequences of up to 7700 tokens and 693
+// rows (16 heads over 8 of 128, e4m3) parts of one length by the longest sequence's, as for three rounds, took 17 %
+// longer, the last round being nearly empty.  So are up to four times as many where a sequence's rows fill less than a
+// tile, so that its tokens alone make its work: 64 sequences of up to 8k tokens with 1 to 3 rows each (32 heads over 8)
+// take 2.6 times as long whole.  A prompt's tiles are better whole, the later ones first (2048 tokens: 27 % longer cut).
 constexpr int kTileRoom = 512, kMostCut = 4 * kTileRoom;
 
 Plan plan_of(int64_t tokens, int n_seqs, bool ragged, int heads, int kv_heads, bool eight, int64_t max_length,

@@ -170,13 +170,21 @@ struct Step {
 };
 
 // The sequence of each lane's row and the row's position there, or a negative position for a row that is padding.
-// The wave searches for its first row; a lane walks on from there, a wave's rows being few.
+// The wave searches for its first row's; a lane goes on from there by steps that double, and back by halves: a wave's rows
+// are few, but between two of them may lie all the sequences of a padded batch that have none.
 __device__ __forceinline__ int locate(const kvsnap_sequences& q, int row, int tokens, int& sequence) {
     sequence = row;
     if (q.query_starts) {
         const int first = __builtin_amdgcn_readfirstlane(row);
         sequence = find_sequence(q.n_seqs, first, [&](int s) { return int64_t(q.query_starts[s]); });
-        while (sequence + 1 < q.n_seqs && q.query_starts[sequence + 1] <= row) ++sequence;
+        int step = 1;
+        for (; step < q.n_seqs - sequence && q.query_starts[sequence + step] <= row; step *= 2) sequence += step;
+        for (int high = min(step, q.n_seqs - sequence); high > 1;) {
+            const int half = high >> 1;
+            const bool passed = q.query_starts[sequence + half] <= row;
+            if (passed) sequence += half;
+            high = passed ? high - half : half;
+        }
     }
     const Rows rows = rows_of(q, sequence, tokens);
     const int i = row - rows.first;

@@ -336,3 +336,72 @@ def test_append_on_a_side_stream_and_captured():
         assert torch.equal(scales.view(torch.uint8), replayed[1])
         lengths += 1
         start = cache.clone(), scales.view(torch.uint8).clone()
+
+
+def padded_batch(live, seqs, held, width=64, heads=3):
+    """A step of ``seqs`` rows and sequences of which ``live``, spread among the others, have a row each (at most two)."""
+    rng = random.Random(live)
+    added = [0] * seqs
+    for s in rng.sample(range(seqs), live):
+        added[s] = rng.choice([1, 1, 2])
+    blocks = seqs + 1
+    cache, scales = make_cache("kv_split", blocks, 16, 1, width, E4M3 if held == "e4m3" else BF16, live)
+    lengths = [n + rng.randrange(12) if n else 0 for n in added]
+    tables, lengths, starts = plan(added, lengths, 16, blocks, live)
+    fused = made((seqs + live, heads + 2, width), BF16, live)
+    return cache, scales, tables, lengths, starts, fused, sum(added)
+
+
+@pytest.mark.parametrize("held", ["16-bit", "e4m3"])
+@pytest.mark.parametrize("live,seqs", [(1, 600), (10, 600), (64, 600), (600, 600), (0, 600)])
+def test_append_of_a_padded_batch_is_its_definition(live, seqs, held):
+    cache, scales, tables, lengths, starts, fused, tokens = padded_batch(live, seqs, held)
+    layer = PagedCache(cache, 16, scales=scales)
+    before, before_scales = cache.clone().cpu(), None if scales is None else scales.clone().cpu()
+    table = table64(64, 40)
+    q, k, v = fused.cuda().split([3, 1, 1], 1)
+    out = torch.full(q.shape, -5.0, dtype=BF16, device="cuda")
+    layer.append(k, v, tables.cuda(), lengths.cuda(), query_starts=starts.cuda(), query=q, rotary=table.float().cuda(),
+                 query_out=out)
+    assert (out[tokens:] == -5).all()
+    added = (starts[1:] - starts[:-1]).tolist()
+    at = torch.cat([torch.arange(int(n) - a, int(n)) for a, n in zip(added, lengths)])
+    q, k, v = (t.cpu()[:tokens] for t in (q, k, v))
+    if tokens:
+        turned = rotate64(q, at, table)
+        close(out[:tokens], turned, rotation_bound(q, turned, BF16))
+    turned = rotate64(k, at, table) if tokens else k.double()
+    slack = [rotation_bound(k, torch.zeros_like(turned), FP32).expand(turned.shape) if tokens else turned,
+             torch.zeros(v.shape).double()]
+    want, bound, bytes_ = expect_append(before, before_scales, k, v, turned, tables, lengths, starts, 16, slack)
+    for side, wanted, off in zip(sides(cache.cpu()), want, bound):
+        close(side.float(), wanted, off)
+    if scales is not None:
+        assert torch.equal(scales.view(torch.uint8).cpu().int(), bytes_)
+
+
+def test_a_padded_batch_takes_no_longer_than_a_full_one():
+    """Ten rows among 4096 sequences: a wave that holds the last of them and padding passes 4000 sequences in a few
+    steps (a walk took 60 times a full batch's time)."""
+    took = []
+    for live in (4096, 10):
+        cache, scales, tables, lengths, starts, fused, _ = padded_batch(live, 4096, "16-bit")
+        if live == 10:              # the ten at the front, as a captured batch has them
+            starts = torch.arange(4097, dtype=torch.int32).clamp(max=10)
+        layer = PagedCache(cache, 16)
+        tables, lengths, starts, (q, k, v) = tables.cuda(), lengths.cuda(), starts.cuda(), fused.cuda().split([3, 1, 1], 1)
+        layer.append(k, v, tables, lengths, query_starts=starts, query=q)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            for _ in range(20):
+                layer.append(k, v, tables, lengths, query_starts=starts, query=q)
+        times = []
+        for _ in range(7):
+            begin, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            begin.record()
+            graph.replay()
+            end.record()
+            torch.cuda.synchronize()
+            times.append(begin.elapsed_time(end))
+        took.append(sorted(times)[3])
+    assert took[1] < 8 * took[0], took

@@ -881,7 +881,7 @@ __global__ __launch_bounds__(kTileWaves * 64, kD <= 128 ? 2 : 1) void attend_til
                 // (32 unsigned bits: the builtin's int would take a place from 32 GiB on as one below the cache)
                 const uint32_t place = __builtin_amdgcn_readlane(places.at, group);
                 const int64_t at = (int64_t(place) << 4) + (first_row & 15) * int64_t(a.token_pieces) * 16;
-                if (kPieces == kBeside || has_piece) {
+                if (has_piece) {
                     load_words<kEight ? 2 : 4>(keys + at + my_offset, k_words[i]);
                     load_words<kEight ? 2 : 4>(values + at + my_offset, v_words[i]);
                 }

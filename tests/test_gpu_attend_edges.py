@@ -227,3 +227,31 @@ def test_cut_rows_and_tiles_of_every_width(width, size, held):
         out, lse = layer.attend(query.cuda(), tables.cuda(), lengths.cuda(), window=window, return_lse=True,
                                 query_starts=None if starts is None else starts.cuda())
         check(out, query, exact, tables, lengths, starts, lse=lse, window=window)
+
+
+@pytest.mark.parametrize("held", ["16-bit", "e4m3"])
+@pytest.mark.parametrize("width", [16, 32, 48, 80, 112, 176, 208, 240])
+def test_tiles_read_no_further_than_a_heads_width(width, held):
+    """Whole stages of 64 tokens that every row sees, at widths that are less than the kernels' own: what lies behind a
+    head's row (another head's of NaN, and behind the cache's last row a tail of NaN) does not reach the head."""
+    size, kv, blocks, length, rows = 16, 2, 20, 320, 40
+    dtype = E4M3 if held == "e4m3" else BF16
+    shape = (2, blocks, size, kv, width)
+    some = made(shape, torch.float32, width).to(dtype)
+    backing = torch.full((some.numel() + 512,), math.nan).to(dtype)
+    cache = backing[:some.numel()].view(shape)
+    cache[:, :, :, 0] = some[:, :, :, 0]
+    on_gpu = backing.cuda()[:some.numel()].view(shape)
+    scales = torch.full((blocks, kv, 2), 127, dtype=torch.uint8) if held == "e4m3" else None
+    layer = PagedCache(on_gpu, size, scales=None if scales is None else scales.cuda())
+    tables = tables_for([length], size, blocks, width, spare=0)
+    lengths, starts = torch.tensor([length], dtype=torch.int32), torch.tensor([0, rows], dtype=torch.int32)
+    query = made((rows, 4, width), BF16, 5)
+    out = layer.attend(query.cuda(), tables.cuda(), lengths.cuda(), query_starts=starts.cuda())
+    assert out[:, 2:].isnan().all()
+    check(out[:, :2], query[:, :2], [side[:, :, :1] for side in dequantised(cache, scales)], tables, lengths, starts)
+    # the other head is the last of its rows
+    cache[:, :, :, 0], cache[:, :, :, 1] = math.nan, some[:, :, :, 1]
+    on_gpu.view(torch.uint8).copy_(cache.view(torch.uint8))
+    out = layer.attend(query.cuda(), tables.cuda(), lengths.cuda(), query_starts=starts.cuda())
+    check(out[:, 2:], query[:, 2:], [side[:, :, 1:] for side in dequantised(cache, scales)], tables, lengths, starts)

@@ -744,7 +744,7 @@ __device__ __forceinline__ uint32_t not_finite(uint32_t word) {
 // meet every bank); V's are 64 or 192 bytes past a multiple of 256, so that the 64 bytes of four rows that half a wave's
 // transposing read takes lie side by side over the banks.  No read waits for a bank.
 //
-// An 8k prompt of 32 heads over 8 of 128 in bf16 takes 638 us, 861 TFLOP/s of the products that its mask leaves, where a
+// An 8k prompt of 32 heads over 8 of 128 in bf16 takes 633 us, 868 TFLOP/s of the products that its mask leaves, where a
 // large plain product reaches 1280 on this card.  A stage costs a wave 1024 cycles of products and about 1100 of vector
 // instructions (32 scores a lane: a multiplication, an exponential, a sum, half a rounding, half a maximum), and the two
 // waves of a SIMD overlap little of the two.  Tried and slower: the next stage's scores between this stage's
